@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libffnk.so"
 CALL_PATH = LIB_PATH.with_name("_call.so")
 
 OP_LINEAR_FWD, OP_FFN_FWD, OP_LINEAR_BWD, OP_FFN_UP, OP_FFN_DOWN, OP_BWD_DX, OP_BWD_DW, OP_FFN_BWD = range(8)
+DT_BF16, DT_FP16, DT_FP32 = range(3)
 PATH_MFMA_TILED, PATH_STREAM, PATH_GENERIC = range(3)
 STATIC_SCRATCH_BYTES = 32 << 20  # FFNK_STATIC_SCRATCH_BYTES
 
@@ -91,6 +92,24 @@ _SIGNATURES = {
 }
 for _name in ("ffnk_masked_linear_fwd", "ffnk_masked_ffn_fwd"):
     _SIGNATURES[f"{_name}_routing"] = _SIGNATURES[f"{_name}_routed"]
+# tensors held in MXFP4 are passed as const ffnk_mxfp4_t*
+_SIGNATURES.update({
+    "ffnk_mxfp4_quantise": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    "ffnk_mxfp4_dequantise": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p]),
+    "ffnk_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
+    "ffnk_mxfp4_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,  # x, xq, Wv, Wt, mask
+                                      c_void_p, c_int64, c_int64, c_int64, c_int64,               # y, M, K, N
+                                      c_void_p, c_size_t, c_void_p, c_void_p]),
+    "ffnk_mxfp4_ffn_fwd": (c_int, [c_void_p, c_int64, c_void_p] + [c_void_p] * 6 + [c_void_p,     # x, xq, weights, mask
+                                   c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,        # out, pre, M, d, h
+                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+    "ffnk_mxfp4_linear_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p,            # g, Wv, Wt, mask
+                                      c_void_p, c_int64, c_int64, c_int64, c_int64,               # dx, M, K, N
+                                      c_void_p, c_size_t, c_void_p, c_void_p]),
+    "ffnk_mxfp4_ffn_bwd": (c_int, [c_void_p, c_int64] + [c_void_p] * 6 + [c_void_p, c_void_p,     # g, weights, mask, pre
+                                   c_void_p, c_int64, c_int64, c_int64, c_int64,                  # dx, M, d, h
+                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+})
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 
@@ -106,6 +125,11 @@ class TileConfig(ctypes.Structure):
 class RoutingStruct(ctypes.Structure):
     """Mirror of ffnk_routing_t: device addresses of perm int32[M] and counts int32[2]."""
     _fields_ = [("perm", c_void_p), ("counts", c_void_p)]
+
+
+class Mxfp4Struct(ctypes.Structure):
+    """Mirror of ffnk_mxfp4_t: device addresses of a tensor's codes and scales."""
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p)]
 
 
 class PartitionStruct(ctypes.Structure):

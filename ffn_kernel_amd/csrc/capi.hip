@@ -8,6 +8,7 @@
 
 #include <atomic>
 
+#include "capi_parts.hpp"
 #include "common.hpp"
 #include "launch.hpp"
 #include "tile_table.hpp"
@@ -1453,3 +1454,101 @@ int ffnk_masked_ffn_bwd_saved(const uint16_t* g, int64_t g_stride_m, const uint1
 }
 
 }  // extern "C"
+
+// ---- what the other files of the C ABI use (capi_parts.hpp) ----
+namespace ffnk {
+
+int api_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int api_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+int api_check_extents(int64_t M, int64_t K, int64_t N) { return check_extents(M, K, N); }
+
+size_t routing_bytes(int64_t M) { return route_ws_bytes(M); }
+int make_routing(const ffnk_routing_t* caller, uint8_t* ws, const uint8_t* mask, int64_t M, hipStream_t stream, const int32_t** perm,
+                 const int32_t** counts) {
+  Routing rt;
+  if (int e = resolve_routing(caller, false, carve_route(ws, M), mask, M, false, stream, &rt)) return e;
+  *perm = rt.perm;
+  *counts = rt.counts;
+  return FFNK_OK;
+}
+
+bool linear_dx_ok(int64_t M, int64_t K, int64_t N, int64_t g_stride_m) {
+  return kmajor_ok(N, K, K, nullptr, nullptr) && direct_ok(N, M, g_stride_m, 8);
+}
+int linear_dx(const uint16_t* g, int64_t g_stride_m, const uint16_t* const (&W)[2], const int32_t* perm, const int32_t* counts, uint16_t* dx,
+              int64_t dx_stride_m, int64_t M, int64_t K, int64_t N, hipStream_t stream) {
+  GemmArgs a;
+  a.A = g; a.lda = g_stride_m;
+  a.B0[0] = W[0]; a.B0[1] = W[1]; a.B1[0] = a.B1[1] = nullptr; a.ldb = K;
+  a.C = dx; a.ldc = dx_stride_m;
+  a.perm = perm; a.counts = counts;
+  a.M = (int)M; a.N = (int)K; a.K = (int)N; a.group_m = plan_group_m(TUNED_NONE, M, N, K);
+  FFNK_HIP(launch_linear_gemm_kmajor(bwd_tile(M, K, N, true), a, stream), "dx GEMM");
+  return FFNK_OK;
+}
+
+namespace {
+struct FfnDxPlan {
+  int64_t half;
+  RoutedPlan dx;
+  size_t dx_need, off_dh, off_p, total;
+};
+FfnDxPlan plan_ffn_dx(int64_t M, int64_t d, int64_t h) {
+  FfnDxPlan p;
+  p.half = round_up64(h, 64);
+  p.dx = ffn_bwd_dx_plan(M, d, 2 * p.half, true, 2 * ws_align((size_t)h * d * 2), &p.dx_need);
+  p.off_dh = ws_align((size_t)M * 2 * p.half * 2);
+  p.off_p = p.off_dh + ws_align((size_t)M * h * 2);
+  p.total = p.off_p + ws_align(p.dx_need);
+  return p;
+}
+}  // namespace
+
+bool ffn_dx_ok(int64_t M, int64_t d, int64_t h, int64_t g_stride_m) {
+  const int64_t half = round_up64(h, 64);
+  return h % 8 == 0 && kmajor_ok(d, h, h, nullptr, nullptr) && direct_ok(d, M, g_stride_m, 8) && kmajor_ok(2 * half, d, d, nullptr, nullptr) &&
+         direct_ok(2 * half, 0, 2 * half, 8);
+}
+size_t ffn_dx_bytes(int64_t M, int64_t d, int64_t h) { return plan_ffn_dx(M, d, h).total; }
+int ffn_dx(const uint16_t* g, int64_t g_stride_m, const uint16_t* pre, const uint16_t* const (&W1)[2], const uint16_t* const (&W3)[2],
+           const uint16_t* const (&W2)[2], const int32_t* perm, const int32_t* counts, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t d, int64_t h,
+           uint8_t* ws, hipStream_t stream) {
+  const FfnDxPlan p = plan_ffn_dx(M, d, h);
+  uint16_t* T13 = reinterpret_cast<uint16_t*>(ws);
+  GemmArgs a;
+  a.A = g; a.lda = g_stride_m;
+  a.B0[0] = W2[0]; a.B0[1] = W2[1]; a.B1[0] = a.B1[1] = nullptr; a.ldb = h;
+  a.C = reinterpret_cast<uint16_t*>(ws + p.off_dh); a.ldc = h;
+  a.perm = perm; a.counts = counts;
+  a.M = (int)M; a.N = (int)h; a.K = (int)d; a.group_m = plan_group_m(TUNED_NONE, M, d, h);
+  a.pre = pre; a.ld_pre = 2 * h; a.half_pre = (int)h;
+  a.T13 = T13; a.ld13 = 2 * p.half; a.half = (int)p.half;
+  FFNK_HIP(launch_gather_gemm_kmajor(bwd_tile(M, h, d, true), a, stream), "dh GEMM");
+  GemmArgs b;
+  b.A = T13; b.lda = 2 * p.half;
+  b.B0[0] = W1[0]; b.B0[1] = W1[1]; b.B1[0] = W3[0]; b.B1[1] = W3[1]; b.ldb = d;
+  b.k_switch = (int)p.half;
+  b.k_rows = (int)h;
+  b.C = dx; b.ldc = dx_stride_m; b.perm = perm; b.counts = counts;
+  b.M = (int)M; b.N = (int)d; b.K = (int)(2 * p.half); b.group_m = plan_group_m(TUNED_NONE, M, 2 * p.half, d);
+  if (p.dx.splits > 1) {
+    b.splits = p.dx.splits;
+    b.splits_more = p.dx.splits_more;
+    b.P = reinterpret_cast<float*>(ws + p.off_p);
+  } else if (p.dx_need > 0) {
+    b.P_tail = reinterpret_cast<float*>(ws + p.off_p);
+  }
+  FFNK_HIP(launch_down_gemm_kmajor(p.dx.tile, b, stream), "dx GEMM");
+  if (p.dx.splits > 1)
+    FFNK_HIP(launch_routed_reduce(b.P, p.dx.splits, p.dx.splits_more, tile_geom(p.dx.tile, false).block_m, (int)M, (int)d, counts, perm, dx, dx_stride_m,
+                                  stream), "dx reduce");
+  return FFNK_OK;
+}
+
+}  // namespace ffnk

@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .mxfp4 import MXFP4, MaskedFFNMXFP4, MaskedLinearMXFP4, mxfp4_quantise
 from .ops import MaskedFFN, MaskedLinear
 
 
@@ -60,3 +61,66 @@ class MaskedFFNModule(nn.Module):
         y = MaskedFFN.apply(x2, self.w1.weight.T, self.w2.weight.T, self.w3.weight.T,
                             self.u1.weight.T, self.u2.weight.T, self.u3.weight.T, m)
         return _unflatten(y, batch)
+
+
+class _MXFP4Weights(nn.Module):
+    """Weights held in MXFP4 as buffers (`<name>_codes`, `<name>_scales`): constants that follow the module to a device and into its
+    state_dict.  Made from a bf16 module with from_module, or empty (zeros) for load_state_dict."""
+
+    def __init__(self, shapes: dict, device=None):
+        super().__init__()
+        self._columns = {name: columns for name, (_, columns) in shapes.items()}
+        self._held = {}
+        for name, (rows, columns) in shapes.items():
+            blocks = -(-columns // 32)
+            self.register_buffer(f"{name}_codes", torch.zeros((rows, 16 * blocks), dtype=torch.uint8, device=device))
+            self.register_buffer(f"{name}_scales", torch.zeros((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device))
+
+    def _quantise(self, weights: dict) -> None:
+        for name, w in weights.items():
+            q = mxfp4_quantise(w)
+            setattr(self, f"{name}_codes", q.codes)
+            setattr(self, f"{name}_scales", q.scales)
+
+    def weight(self, name: str) -> MXFP4:
+        codes, scales = self._buffers[f"{name}_codes"], self._buffers[f"{name}_scales"]
+        held = self._held.get(name)
+        if held is None or held.codes is not codes or held.scales is not scales:
+            held = self._held[name] = MXFP4(codes, scales, self._columns[name])
+        return held
+
+
+class MaskedLinearMXFP4Module(_MXFP4Weights):
+    """MaskedLinearModule over weights in MXFP4; its rows are differentiable, its weights constants."""
+
+    def __init__(self, in_dim: int, out_dim: int, device=None):
+        super().__init__({"linear_v": (out_dim, in_dim), "linear_t": (out_dim, in_dim)}, device)
+
+    @classmethod
+    def from_module(cls, m: MaskedLinearModule) -> "MaskedLinearMXFP4Module":
+        new = cls(m.linear_v.in_features, m.linear_v.out_features, device="meta")
+        new._quantise({"linear_v": m.linear_v.weight, "linear_t": m.linear_t.weight})
+        return new
+
+    def forward(self, x: torch.Tensor, visual_mask: torch.Tensor) -> torch.Tensor:
+        x2, m, batch = _flatten(x, visual_mask)
+        return _unflatten(MaskedLinearMXFP4.apply(x2, self.weight("linear_v"), self.weight("linear_t"), m), batch)
+
+
+class MaskedFFNMXFP4Module(_MXFP4Weights):
+    """MaskedFFNModule over weights in MXFP4; its rows are differentiable, its weights constants."""
+    _NAMES = ("w1", "w2", "w3", "u1", "u2", "u3")
+
+    def __init__(self, hidden_size: int, intermediate_size: int, device=None):
+        up, down = (intermediate_size, hidden_size), (hidden_size, intermediate_size)
+        super().__init__({name: down if name[1] == "2" else up for name in self._NAMES}, device)
+
+    @classmethod
+    def from_module(cls, m: MaskedFFNModule) -> "MaskedFFNMXFP4Module":
+        new = cls(m.w1.in_features, m.w1.out_features, device="meta")
+        new._quantise({name: getattr(m, name).weight for name in cls._NAMES})
+        return new
+
+    def forward(self, x: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
+        x2, m, batch = _flatten(x, mask)
+        return _unflatten(MaskedFFNMXFP4.apply(x2, *(self.weight(name) for name in self._NAMES), m), batch)

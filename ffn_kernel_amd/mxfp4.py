@@ -1,0 +1,347 @@
+"""The routed layers over weights held in 4 bits (MXFP4, OCP Microscaling): quantisation, MaskedLinear and MaskedFFN.
+
+    q = mxfp4_quantise(weight)                          # nn.Linear.weight [out, in], blocks of 32 along `in`
+    MaskedLinearMXFP4.apply(a, b1, b2, mask) -> c       # MaskedLinear with b1, b2 the quantised weights (not transposed views)
+    MaskedFFNMXFP4.apply(a, w1, w2, w3, u1, u2, u3, mask)
+
+A block of 32 columns shares a power of two; its elements are 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign.  The rows `a` (bf16) are
+quantised the same way in the call, and so is the SwiGLU intermediate, so that the matrix cores multiply 4-bit operands; sums are
+held in fp32.  `a` may also be an MXFP4 tensor: rows that several projections share are quantised once.
+
+The weights are constants.  The gradient of `a` passes the quantisations over (straight-through), which is what training adapters
+over a frozen model asks for.  No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import (Routing, _grad_mode, _on_device, _require_cuda_bf16, _require_mask, _route_cache, _routing_arg, _same_device,
+                  _stream_ptr, _workspace)
+
+_BLOCK = 32
+_DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_FP16, torch.float32: _lib.DT_FP32}
+
+
+def _code_bytes(columns: int) -> int:
+    return -(-columns // _BLOCK) * 16
+
+
+def _scale_bytes(columns: int) -> int:
+    return -(-columns // (_BLOCK * 16)) * 16
+
+
+class MXFP4:
+    """A [rows, columns] tensor in MXFP4 on a GPU: `codes` uint8 [rows, 16 ceil(columns / 32)], two elements to a byte with the even
+    column in the low half, and `scales` uint8 [rows, a multiple of 16], one exponent byte (bias 127) for 32 columns.  Bytes past the
+    last column and the last block are 0: mxfp4_quantise and from_parts see to that, and the products count on it."""
+    __slots__ = ("_codes", "_scales", "_columns", "_struct", "_address")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
+        for name, t, width in (("codes", codes, _code_bytes(columns)), ("scales", scales, _scale_bytes(columns))):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != width:
+                raise ValueError(f"{name} must be a torch.uint8 tensor [rows, {width}] for {columns} columns")
+            if not t.is_cuda:
+                raise ValueError(f"{name} must live on a GPU (got {t.device}); libffnk has no CPU path")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+        if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
+            raise ValueError(f"codes are {tuple(codes.shape)} on {codes.device}, scales {tuple(scales.shape)} on {scales.device}")
+        self._codes, self._scales, self._columns = codes, scales, int(columns)
+        self._struct = _lib.Mxfp4Struct(codes.data_ptr(), scales.data_ptr())
+        self._address = ctypes.addressof(self._struct)
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int | None = None) -> "MXFP4":
+        """From codes [rows, at least ceil(columns / 2)] and scales [rows, at least ceil(columns / 32)] (uint8 or float8_e8m0fnu) as
+        checkpoints hold them; columns: two for each byte of codes where it is not given.  Copies both."""
+        scales = scales.view(torch.uint8)
+        if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[0] != scales.shape[0]:
+            raise ValueError(f"codes and scales must be 8-bit [rows, ...] tensors, got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        rows, columns = codes.shape[0], 2 * codes.shape[1] if columns is None else int(columns)
+        held, blocks = -(-columns // 2), -(-columns // _BLOCK)
+        if columns < 0 or codes.shape[1] < held or scales.shape[1] < blocks:
+            raise ValueError(f"{columns} columns need {held} bytes of codes and {blocks} scales a row, got {codes.shape[1]} and {scales.shape[1]}")
+        new_codes = torch.zeros((rows, _code_bytes(columns)), dtype=torch.uint8, device=codes.device)
+        new_scales = torch.zeros((rows, _scale_bytes(columns)), dtype=torch.uint8, device=codes.device)
+        new_codes[:, :held] = codes[:, :held]
+        if columns % 2:
+            new_codes[:, held - 1] &= 15
+        new_scales[:, :blocks] = scales[:, :blocks]
+        return cls(new_codes, new_scales, columns)
+
+    def __reduce__(self):
+        return MXFP4, (self._codes, self._scales, self._columns)
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    columns = property(lambda self: self._columns)
+    rows = property(lambda self: self._codes.shape[0])
+    shape = property(lambda self: (self._codes.shape[0], self._columns))
+    device = property(lambda self: self._codes.device)
+
+    def dequantise(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        return mxfp4_dequantise(self, dtype)
+
+    def __repr__(self):
+        return f"MXFP4(shape={self.shape}, device='{self.device}')"
+
+
+def _require_mxfp4(name: str, q) -> None:
+    if not isinstance(q, MXFP4):
+        raise TypeError(f"{name} must be an MXFP4 tensor (mxfp4_quantise), got {type(q).__name__}")
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    """[M, K] rows with unit column stride that do not overlap; anything else is copied once."""
+    M, K = t.shape
+    return t if (K <= 1 or t.stride(1) == 1) and (M <= 1 or t.stride(0) >= K) else t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
+    """The rows of `t` ([rows, columns], bf16, fp16 or fp32) in MXFP4, in blocks of 32 columns (ffnk_mxfp4_quantise): the scale is the
+    largest power of two not above the block's largest magnitude, over 4; elements go to the nearest number, ties to the even code,
+    and saturate at 6.  A block with an infinity or a NaN is NaN.  The result carries no gradient."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"t must be a torch.Tensor, got {type(t).__name__}")
+    if t.dim() != 2 or t.dtype not in _DTYPES:
+        raise ValueError(f"t must be a 2-D bf16, fp16 or fp32 tensor, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"t must live on a GPU (got {t.device}); libffnk has no CPU path")
+    t = _dense_rows(t.detach())
+    rows, columns = t.shape
+    with _on_device(t.device):
+        codes = torch.empty((rows, _code_bytes(columns)), dtype=torch.uint8, device=t.device)
+        scales = torch.empty((rows, _scale_bytes(columns)), dtype=torch.uint8, device=t.device)
+        q = MXFP4(codes, scales, columns)
+        _lib.check(_lib.load().ffnk_mxfp4_quantise(t.data_ptr(), _DTYPES[t.dtype], _row_stride(t), q._address, rows, columns,
+                                                   _stream_ptr(t.device)), "ffnk_mxfp4_quantise")
+    return q
+
+
+def mxfp4_dequantise(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that `q` stands for, as a [rows, columns] tensor of bf16 (exact for normal numbers), fp16 or fp32."""
+    _require_mxfp4("q", q)
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+    rows, columns = q.shape
+    with _on_device(q.device):
+        t = torch.empty((rows, columns), dtype=dtype, device=q.device)
+        _lib.check(_lib.load().ffnk_mxfp4_dequantise(q._address, t.data_ptr(), _DTYPES[dtype], max(columns, 1), rows, columns,
+                                                     _stream_ptr(q.device)), "ffnk_mxfp4_dequantise")
+    return t
+
+
+def _mx_workspace(op: int, M: int, K: int, N: int, dev: torch.device) -> torch.Tensor:
+    n = _lib.load().ffnk_mxfp4_workspace_bytes(op, M, K, N)
+    if n == ctypes.c_size_t(-1).value:
+        raise ValueError(f"ffnk_mxfp4_workspace_bytes: invalid op/extents op={op} M={M} K={K} N={N}")
+    return _workspace(n, dev)
+
+
+def _rows_of_call(a):
+    """(a as the kernels take it, address of its bf16 rows, their stride, address of its MXFP4 struct): one of the two is there."""
+    if isinstance(a, MXFP4):
+        return a, None, 0, a._address
+    _require_cuda_bf16("a", a, 2)
+    a = _dense_rows(a)
+    return a, a.data_ptr(), _row_stride(a), None
+
+
+def _check_weights(K: int, dev, shape, **weights) -> None:
+    for name, w in weights.items():
+        _require_mxfp4(name, w)
+        if w.shape != shape:
+            raise ValueError(f"{name} shape {w.shape} != {shape}")
+    _same_device(dev, **weights)
+
+
+def _check_differentiable(contraction: int, *extents: int) -> None:
+    """What the backward GEMMs over dequantised weights take; `contraction`: the layer's output features."""
+    if any(e % 8 for e in (contraction, *extents)) or (contraction % 64 and contraction < 128):
+        raise ValueError(f"the MXFP4 backward needs extents that are multiples of 8 and output features that are a multiple of 64 or at "
+                         f"least 128, got {(contraction, *extents)}")
+
+
+def masked_linear_mxfp4_forward(a, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
+    """c[m] = Q(a[m]) @ (b1 if mask[m] else b2)^T.  a: bf16 [M, K] or MXFP4; b1, b2: MXFP4 [N, K]; routing: as in
+    masked_linear_forward."""
+    a, x, ld, xq = _rows_of_call(a)
+    M, K = a.shape
+    dev = a.device
+    _require_mxfp4("b1", b1)
+    N = b1.rows
+    _check_weights(K, dev, (N, K), b1=b1, b2=b2)
+    mask = _require_mask(mask, M, dev)
+    with _on_device(dev):
+        c = torch.empty((M, N), device=dev, dtype=torch.bfloat16)
+        if M == 0 or N == 0 or K == 0:
+            return c.zero_()
+        stream = _stream_ptr(dev)
+        routing, rt = _routing_arg(routing, mask, M, stream)
+        ws = _mx_workspace(_lib.OP_LINEAR_FWD, M, K, N, dev)
+        rc = _lib.load().ffnk_mxfp4_linear_fwd(x, ld, xq, b1._address, b2._address, mask.data_ptr(), c.data_ptr(), N, M, K, N, ws.data_ptr(),
+                                               ws.numel(), stream, rt)
+    _lib.check(rc, "ffnk_mxfp4_linear_fwd")
+    return c
+
+
+def masked_linear_mxfp4_backward(grad: torch.Tensor, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
+    """da[m] = grad[m] @ (b1 if mask[m] else b2): the gradient of the rows over constant weights."""
+    _require_cuda_bf16("grad", grad, 2)
+    _require_mxfp4("b1", b1)
+    M, dev = grad.shape[0], grad.device
+    N, K = b1.shape
+    if grad.shape != (M, N):
+        raise ValueError(f"grad shape {tuple(grad.shape)} != {(M, N)}")
+    _check_weights(K, dev, (N, K), b1=b1, b2=b2)
+    _check_differentiable(N, K)
+    mask = _require_mask(mask, M, dev)
+    grad = _aligned_rows(grad)
+    with _on_device(dev):
+        da = torch.empty((M, K), device=dev, dtype=torch.bfloat16)
+        if M == 0 or K == 0 or N == 0:
+            return da.zero_()
+        stream = _stream_ptr(dev)
+        routing, rt = _routing_arg(routing, mask, M, stream)
+        ws = _mx_workspace(_lib.OP_LINEAR_BWD, M, K, N, dev)
+        rc = _lib.load().ffnk_mxfp4_linear_bwd(grad.data_ptr(), _row_stride(grad), b1._address, b2._address, mask.data_ptr(), da.data_ptr(), K,
+                                               M, K, N, ws.data_ptr(), ws.numel(), stream, rt)
+    _lib.check(rc, "ffnk_mxfp4_linear_bwd")
+    return da
+
+
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows of a multiple of 8 columns that the direct kernels load as they are; others are copied."""
+    t = _dense_rows(t)
+    return t if _row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _check_ffn(a_shape, dev, w1, w2, w3, u1, u2, u3):
+    d = a_shape[1]
+    _require_mxfp4("w1", w1)
+    h = w1.rows
+    _check_weights(d, dev, (h, d), w1=w1, w3=w3, u1=u1, u3=u3)
+    _check_weights(h, dev, (d, h), w2=w2, u2=u2)
+    return d, h
+
+
+def masked_ffn_mxfp4_forward(a, w1: MXFP4, w2: MXFP4, w3: MXFP4, u1: MXFP4, u2: MXFP4, u3: MXFP4, mask: torch.Tensor, save_pre: bool = False,
+                             routing: Routing | None = None):
+    """Q(silu(Q(a) @ w1^T) * (Q(a) @ w3^T)) @ w2^T for rows with mask, u1, u2, u3 for the others.  a: bf16 [M, d] or MXFP4;
+    w1, w3, u1, u3: MXFP4 [h, d]; w2, u2: MXFP4 [d, h].
+
+    save_pre: also return both projections, bf16 [M, 2h] in routed order (gate | up), for masked_ffn_mxfp4_backward."""
+    a, x, ld, xq = _rows_of_call(a)
+    M, dev = a.shape[0], a.device
+    d, h = _check_ffn(a.shape, dev, w1, w2, w3, u1, u2, u3)
+    mask = _require_mask(mask, M, dev)
+    with _on_device(dev):
+        out = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
+        pre = torch.empty((M, 2 * h), device=dev, dtype=torch.bfloat16) if save_pre else None
+        if M == 0 or d == 0 or h == 0:
+            return (out.zero_(), pre) if save_pre else out.zero_()
+        stream = _stream_ptr(dev)
+        routing, rt = _routing_arg(routing, mask, M, stream)
+        ws = _mx_workspace(_lib.OP_FFN_FWD, M, d, h, dev)
+        rc = _lib.load().ffnk_mxfp4_ffn_fwd(x, ld, xq, w1._address, w2._address, w3._address, u1._address, u2._address, u3._address, mask.data_ptr(),
+                                            out.data_ptr(), d, pre.data_ptr() if save_pre else None, M, d, h, ws.data_ptr(), ws.numel(), stream, rt)
+    _lib.check(rc, "ffnk_mxfp4_ffn_fwd")
+    return (out, pre) if save_pre else out
+
+
+def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP4, u1: MXFP4, u2: MXFP4, u3: MXFP4, mask: torch.Tensor,
+                              pre: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
+    """Gradient of the rows over constant weights: dh = grad @ w2, da = (dh * up * silu'(gate)) @ w1 + (dh * silu(gate)) @ w3, with the
+    projections that masked_ffn_mxfp4_forward(..., save_pre=True) returned for the same mask."""
+    _require_cuda_bf16("grad", grad, 2)
+    M, dev = grad.shape[0], grad.device
+    d, h = _check_ffn(grad.shape, dev, w1, w2, w3, u1, u2, u3)
+    _check_differentiable(d, h)
+    mask = _require_mask(mask, M, dev)
+    _require_cuda_bf16("pre", pre, 2)
+    if pre.shape != (M, 2 * h) or pre.device != dev or not pre.is_contiguous() or pre.data_ptr() % 16:
+        raise ValueError(f"pre must be a contiguous, 16-byte aligned bf16 [{M}, {2 * h}] tensor on {dev}")
+    grad = _aligned_rows(grad)
+    with _on_device(dev):
+        da = torch.empty((M, d), device=dev, dtype=torch.bfloat16)
+        if M == 0 or d == 0 or h == 0:
+            return da.zero_()
+        stream = _stream_ptr(dev)
+        routing, rt = _routing_arg(routing, mask, M, stream)
+        ws = _mx_workspace(_lib.OP_FFN_BWD, M, d, h, dev)
+        rc = _lib.load().ffnk_mxfp4_ffn_bwd(grad.data_ptr(), _row_stride(grad), w1._address, w2._address, w3._address, u1._address, u2._address,
+                                            u3._address, mask.data_ptr(), pre.data_ptr(), da.data_ptr(), d, M, d, h, ws.data_ptr(), ws.numel(),
+                                            stream, rt)
+    _lib.check(rc, "ffnk_mxfp4_ffn_bwd")
+    return da
+
+
+class _FrozenWeights(Function):
+    """Notes whether a gradient can be asked for: forward() itself always runs with gradients off."""
+
+    @classmethod
+    def apply(cls, *args):
+        _grad_mode.enabled = torch.is_grad_enabled()
+        return super().apply(*args)
+
+    @staticmethod
+    def _wanted(ctx) -> bool:
+        return _grad_mode.enabled and ctx.needs_input_grad[0]
+
+
+class MaskedLinearMXFP4(_FrozenWeights):
+    """c = Q(a) @ (b1 where mask else b2)^T over MXFP4 weights [N, K]; differentiable in a bf16 `a`."""
+
+    @staticmethod
+    def forward(ctx, a, b1, b2, mask):
+        wanted = _FrozenWeights._wanted(ctx)
+        if wanted and isinstance(b1, MXFP4):
+            _check_differentiable(*b1.shape)
+        _route_cache.last = None
+        out = masked_linear_mxfp4_forward(a, b1, b2, mask)
+        if wanted:
+            ctx.save_for_backward(mask)
+            ctx.weights = (b1, b2)
+            ctx.routing = _route_cache.last
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        mask, = ctx.saved_tensors
+        return masked_linear_mxfp4_backward(grad, *ctx.weights, mask, routing=ctx.routing), None, None, None
+
+
+class MaskedFFNMXFP4(_FrozenWeights):
+    """Routed SwiGLU FFN over MXFP4 weights (w1, w3, u1, u3: [h, d]; w2, u2: [d, h]); differentiable in a bf16 `a`, for which the
+    forward keeps both projections in bf16."""
+
+    @staticmethod
+    def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
+        weights = (w1, w2, w3, u1, u2, u3)
+        wanted = _FrozenWeights._wanted(ctx)
+        if wanted and isinstance(w2, MXFP4):
+            _check_differentiable(*w2.shape)
+        _route_cache.last = None
+        if not wanted:
+            return masked_ffn_mxfp4_forward(a, *weights, mask)
+        out, pre = masked_ffn_mxfp4_forward(a, *weights, mask, save_pre=True)
+        ctx.save_for_backward(mask, pre)
+        ctx.weights = weights
+        ctx.routing = _route_cache.last
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        mask, pre = ctx.saved_tensors
+        return (masked_ffn_mxfp4_backward(grad, *ctx.weights, mask, pre, routing=ctx.routing), *([None] * 7))

@@ -433,6 +433,66 @@ FFNK_API int ffnk_masked_ffn_bwd_routed(const uint16_t* g, int64_t g_stride_m,
                                int64_t M, int64_t d, int64_t h,
                                void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
 
+/* ---------------------------------------------------------------------------------------------------------------------------
+ * MXFP4 (OCP Microscaling): the routed layers over weights, and token rows, held in 4 bits.  No counterpart in the reference.
+ *
+ * A tensor of [rows, columns] holds its rows in blocks of 32 columns, nb = ceil(columns / 32) of them.  An element is
+ * E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times the block's scale, 2^(byte - 127) (E8M0; byte 255: the block is NaN).
+ *   codes:  rows of 16 * nb bytes, two elements to a byte, the even column in the low half; 0 behind the last column
+ *   scales: rows of 16 * ceil(nb / 16) bytes, one for each block; 0 behind the last block (the products rely on it)
+ * Rows follow one another without gaps; both pointers are 16-byte aligned device memory.
+ */
+typedef struct ffnk_mxfp4_t {
+  const uint8_t* codes;
+  const uint8_t* scales;
+} ffnk_mxfp4_t;
+
+/* element types of ffnk_mxfp4_quantise / _dequantise */
+enum { FFNK_DT_BF16 = 0, FFNK_DT_FP16 = 1, FFNK_DT_FP32 = 2 };
+
+/* x [rows, columns] (columns contiguous, row stride x_stride_m elements) -> *out, whose memory is written.  A block's scale is the
+ * largest power of two not above its largest magnitude, over 4 (at least 2^-127); elements are rounded to the nearest number,
+ * ties to the even code, and saturate at 6.  A block with an infinity or a NaN becomes NaN. */
+FFNK_API int ffnk_mxfp4_quantise(const void* x, int dtype, int64_t x_stride_m, const ffnk_mxfp4_t* out, int64_t rows,
+                                 int64_t columns, void* stream);
+/* The values that *x stands for, rounded to dtype (bf16 holds them exactly down to its smallest normal number). */
+FFNK_API int ffnk_mxfp4_dequantise(const ffnk_mxfp4_t* x, void* y, int dtype, int64_t y_stride_m, int64_t rows, int64_t columns,
+                                   void* stream);
+
+/* Scratch of the calls below (op: FFNK_OP_LINEAR_FWD, FFNK_OP_FFN_FWD, FFNK_OP_LINEAR_BWD, FFNK_OP_FFN_BWD; K = d, N = h for the
+ * FFN).  (size_t)-1 for another op or invalid extents. */
+FFNK_API size_t ffnk_mxfp4_workspace_bytes(int op, int64_t M, int64_t K, int64_t N);
+
+/* y[m] = Q(x[m]) (mask[m] ? Wv : Wt)^T with the weights [N, K], as nn.Linear holds them.  The rows are bf16 x, quantised in the
+ * call, or MXFP4 xq (the other is NULL).  fp32 sums, bf16 result.  routing as in ffnk_masked_linear_fwd_routed (M > 64). */
+FFNK_API int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq,
+                                   const ffnk_mxfp4_t* Wv, const ffnk_mxfp4_t* Wt, const uint8_t* mask,
+                                   uint16_t* y, int64_t y_stride_m, int64_t M, int64_t K, int64_t N,
+                                   void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+
+/* out[m] = Q(silu(Q(x[m]) W1^T) * (Q(x[m]) W3^T)) W2^T for visual rows, U1, U2, U3 for text rows; W1, W3 [h, d], W2 [d, h].
+ * The intermediate goes from fp32 straight to MXFP4.  pre (optional, bf16 [M, 2h], 16-byte aligned where a backward reads it):
+ * both projections in routed order, as ffnk_masked_ffn_fwd_save writes them. */
+FFNK_API int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq,
+                                const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
+                                const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
+                                uint16_t* out, int64_t out_stride_m, uint16_t* pre, int64_t M, int64_t d, int64_t h,
+                                void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+
+/* Gradient of the rows over constant weights, the quantisations passed over (straight-through): dx[m] = g[m] W_grp.
+ * K, N multiples of 8, N a multiple of 64 or at least 128; 16-byte aligned rows of g. */
+FFNK_API int ffnk_mxfp4_linear_bwd(const uint16_t* g, int64_t g_stride_m, const ffnk_mxfp4_t* Wv, const ffnk_mxfp4_t* Wt,
+                                   const uint8_t* mask, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t K, int64_t N,
+                                   void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+
+/* The same for the FFN: dh = g W2, dx = (dh * up * silu'(gate)) W1 + (dh * silu(gate)) W3 with the gate | up of `pre`.
+ * d, h multiples of 8, d a multiple of 64 or at least 128; 16-byte aligned rows of g. */
+FFNK_API int ffnk_mxfp4_ffn_bwd(const uint16_t* g, int64_t g_stride_m,
+                                const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
+                                const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
+                                const uint16_t* pre, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t d, int64_t h,
+                                void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,340 @@
+"""MXFP4 operators on the GPU against the 64-bit oracle, element by element within its error bounds: tail blocks, odd extents, row
+counts either side of every path, one modality alone, strides, infinities and NaN, both forms of the rows, gradients, graphs, modules."""
+import copy
+
+import pytest
+import torch
+
+import ffn_kernel_amd as F
+from oracle import mxfp4 as ref
+from tests.helpers import note
+
+pytestmark = pytest.mark.gpu
+FFN = ("w1", "w2", "w3", "u1", "u2", "u3")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rows(m, k, seed, dtype=torch.bfloat16):
+    """Rows with some large channels and some whole blocks of zeros."""
+    g = gen(seed)
+    t = torch.randn(m, k, generator=g, device="cuda")
+    t *= 1 + 15 * (torch.rand(k, generator=g, device="cuda") < 0.02)
+    if k > 64:
+        t[::3, 32:64] = 0
+    return t.to(dtype)
+
+
+def weight(n, k, seed, std=0.05):
+    return (torch.randn(n, k, generator=gen(seed), device="cuda") * std).bfloat16()
+
+
+def a_mask(m, kind, seed=0):
+    if kind in ("visual", "text"):
+        return torch.full((m,), kind == "visual", device="cuda")
+    return torch.rand(m, generator=gen(seed + 77), device="cuda") < 0.4
+
+
+def within(got, value, bound, what):
+    got = got.double()
+    assert got.shape == value.shape, what
+    assert torch.equal(got.isnan(), value.isnan()), f"{what}: NaN elsewhere"
+    excess = ((got - value).abs() / (bound + 1e-300)).nan_to_num(0.0)
+    at = excess.argmax().item() if excess.numel() else 0
+    assert excess.numel() == 0 or excess.max().item() <= 1.0, f"{what}: {excess.max().item():.3f} of the bound at {at}: {got.flatten()[at].item()} for {value.flatten()[at].item()}"
+
+
+# ---- quantisation: codes, scales and values are exact -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 32), (2, 31), (3, 33), (5, 100), (8, 4096), (7, 1544), (65, 2056), (1, 40000), (300, 8), (2500, 4104), (1030, 8192)])
+def test_quantise_is_exact(m, k, dtype):
+    note(f"quantise {m}x{k} {dtype}")
+    t = rows(m, k, m + k, dtype)
+    if k > 8:  # values on the borders of the grid, both zeros, tiny ones
+        t[0, :8] = torch.tensor([6.0, 0.25, -0.75, 2.5, -5.0, 1.25, -0.0, 2.0 ** -20], dtype=dtype)
+    q = F.mxfp4_quantise(t)
+    codes, scales = ref.pack(t)
+    nb = scales.shape[1]
+    assert torch.equal(q.scales[:, :nb], scales) and not q.scales[:, nb:].any()
+    sign = lambda c: torch.where((c & 7) == 0, c & 7, c)  # (a zero's sign is free)
+    assert torch.equal(sign(q.codes & 15), sign(codes & 15)) and torch.equal(sign(q.codes >> 4), sign(codes >> 4))
+    for out in (torch.bfloat16, torch.float16, torch.float32):
+        assert torch.equal(F.mxfp4_dequantise(q, out), ref.values(t).to(out))
+    again = F.MXFP4.from_parts(codes[:, :(k + 1) // 2], scales, k)
+    assert torch.equal(again.dequantise(torch.float32), q.dequantise(torch.float32)) and again.shape == (m, k)
+
+
+def test_quantise_extremes():
+    note("quantise extremes")
+    t = torch.zeros(6, 96, device="cuda")
+    t[0, 5], t[1, 40], t[2, 70] = float("inf"), float("nan"), -float("inf")
+    t[3, :3] = torch.tensor([2.0 ** 127, -(2.0 ** 127) * 1.99, 2.0 ** 125])
+    t[4, :3] = torch.tensor([2.0 ** -126, -(2.0 ** -127), 2.0 ** -149])
+    t[5, 32:35] = torch.tensor([2.0 ** -124, 1.5 * 2.0 ** -126, -(2.0 ** -125)])
+    q = F.mxfp4_quantise(t)
+    assert torch.equal(q.scales[:, :3], ref.pack(t)[1])
+    v, w = F.mxfp4_dequantise(q, torch.float32), ref.values(t).float()
+    assert torch.equal(v.isnan(), w.isnan()) and torch.equal(v.nan_to_num(0.0), w.nan_to_num(0.0))
+    assert v[0, :32].isnan().all() and not v[0, 32:].isnan().any()
+
+
+def test_quantise_reads_rows_as_they_lie():
+    note("quantise strides")
+    big = rows(40, 300, 5)
+    for view in (big[:, :200], big[::2], big[3:, 7:207], big.T, big[:1].expand(9, 300), big[:, ::3], big[:, :0], big[:0]):
+        q = F.mxfp4_quantise(view)
+        assert q.shape == tuple(view.shape) and torch.equal(q.dequantise(torch.float32), ref.values(view).float())
+    p = torch.nn.Parameter(big.clone())
+    assert not F.mxfp4_quantise(p).dequantise().requires_grad
+
+
+# ---- the linear layer -----------------------------------------------------------------------------------------------------------
+
+def linear_case(m, k, n, kind, seed=1):
+    x, wv, wt, mask = rows(m, k, seed), weight(n, k, seed + 1), weight(n, k, seed + 2), a_mask(m, kind, seed)
+    return x, F.mxfp4_quantise(wv), F.mxfp4_quantise(wt), mask, (ref.values(x), ref.values(wv), ref.values(wt))
+
+
+@pytest.mark.parametrize("kind", ["mixed", "visual", "text"])
+@pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 32, 16), (2, 33, 7), (3, 4096, 130), (8, 1024, 1024), (15, 520, 33), (16, 512, 64), (17, 544, 31), (27, 2056, 200),
+                                   (33, 100, 48), (48, 1000, 96), (49, 7168, 65), (64, 1544, 257), (64, 256, 512), (65, 40, 24), (65, 1, 3), (66, 256, 31),
+                                   (100, 264, 129), (127, 512, 128), (130, 1544, 260), (257, 768, 384), (300, 96, 1030), (300, 8192, 256), (513, 1032, 520)])
+def test_linear_forward(m, k, n, kind):
+    note(f"linear {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    value, bound = ref.linear(a, wv, wt, mask)
+    y = F.MaskedLinearMXFP4.apply(x, qv, qt, mask)
+    within(y, value, bound, "rows in bf16")
+    within(F.masked_linear_mxfp4_forward(F.mxfp4_quantise(x), qv, qt, mask), value, bound, "rows in MXFP4")
+    assert torch.equal(y, F.MaskedLinearMXFP4.apply(x, qv, qt, mask)), "the same call twice"
+
+
+@pytest.mark.parametrize("m,k,n,kind", [(2100, 1024, 4160, "mixed"), (4097, 296, 4100, "mixed"), (3000, 520, 8200, "visual"), (2048, 768, 6144, "text"), (70000, 64, 72, "mixed")])
+def test_linear_forward_on_large_tiles(m, k, n, kind):
+    note(f"linear large {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    value, bound = ref.linear(a, wv, wt, mask)
+    within(F.masked_linear_mxfp4_forward(x, qv, qt, mask), value, bound, "rows in bf16")
+    within(F.masked_linear_mxfp4_forward(F.mxfp4_quantise(x), qv, qt, mask), value, bound, "rows in MXFP4")
+
+
+@pytest.mark.parametrize("m", [5, 64, 65, 300])
+def test_linear_infinities_stay_in_their_rows(m):
+    note(f"linear inf / nan {m}")
+    x, qv, qt, mask, (_, wv, wt) = linear_case(m, 512, 96, "mixed")
+    x[1, 300], x[m - 1, 2] = float("inf"), float("nan")
+    value, bound = ref.linear(ref.values(x).nan_to_num(0.0), wv, wt, mask)
+    value[1], value[m - 1] = float("nan"), float("nan")
+    within(F.masked_linear_mxfp4_forward(x, qv, qt, mask), value, bound, "rows with an infinity or a NaN are NaN, the others not")
+
+
+def test_linear_infinite_weights_reach_their_modality_only():
+    note("linear inf weights")
+    for m in (20, 200):
+        x, _, qt, mask, (a, wv, wt) = linear_case(m, 256, 64, "mixed")
+        bad = weight(64, 256, 2)
+        bad[5, 7] = float("inf")
+        value, bound = ref.linear(a, ref.values(bad).nan_to_num(0.0), wt, mask)
+        value[mask, 5] = float("nan")
+        within(F.masked_linear_mxfp4_forward(x, F.mxfp4_quantise(bad), qt, mask), value, bound, "column 5 of the visual rows")
+
+
+@pytest.mark.parametrize("m", [9, 100])
+def test_linear_views_routing_and_empty_calls(m):
+    note(f"linear views {m}")
+    wide, qv, qt, mask, (a, wv, wt) = linear_case(m, 300, 72, "mixed")
+    x = wide[:, 4:260]
+    qv, qt = F.mxfp4_quantise(weight(72, 256, 8)), F.mxfp4_quantise(weight(72, 256, 9))
+    value, bound = ref.linear(ref.values(x), qv.dequantise(torch.float32).double(), qt.dequantise(torch.float32).double(), mask)
+    strided = torch.zeros(m, 3, dtype=torch.bool, device="cuda")
+    strided[:, 1] = mask
+    within(F.masked_linear_mxfp4_forward(x, qv, qt, strided[:, 1]), value, bound, "views")
+    within(F.masked_linear_mxfp4_forward(x, qv, qt, mask, routing=F.route(mask)), value, bound, "a partition made earlier")
+    within(F.masked_linear_mxfp4_forward(x[:1].expand(m, 256), qv, qt, mask), *ref.linear(ref.values(x[:1].expand(m, 256)), qv.dequantise(torch.float32).double(), qt.dequantise(torch.float32).double(), mask), "one row repeated")
+    assert F.masked_linear_mxfp4_forward(x[:0], qv, qt, mask[:0]).shape == (0, 72)
+    with pytest.raises(ValueError, match="routing"):
+        F.masked_linear_mxfp4_forward(x, qv, qt, mask, routing=F.route(mask[:-1]))
+
+
+def test_refusals_on_the_gpu():
+    note("refusals")
+    x, qv, qt, mask, _ = linear_case(8, 64, 32, "mixed")
+    other, up = F.mxfp4_quantise(weight(32, 96, 4)), F.mxfp4_quantise(weight(96, 64, 4))
+    for call in (lambda: F.MaskedLinearMXFP4.apply(x, qv, other, mask), lambda: F.MaskedLinearMXFP4.apply(x, other, other, mask),
+                 lambda: F.MaskedLinearMXFP4.apply(x.float(), qv, qt, mask), lambda: F.MaskedLinearMXFP4.apply(x[0], qv, qt, mask),
+                 lambda: F.MaskedLinearMXFP4.apply(x, qv, qt, mask[:-1]), lambda: F.MaskedLinearMXFP4.apply(x, qv, qt, mask.int()),
+                 lambda: F.MaskedLinearMXFP4.apply(x, qv, qt, mask.cpu()), lambda: F.MaskedLinearMXFP4.apply(x.cpu(), qv, qt, mask),
+                 lambda: F.MaskedFFNMXFP4.apply(x, up, up, up, up, up, up, mask), lambda: F.mxfp4_dequantise(qv, torch.float64),
+                 lambda: F.MXFP4(qv.codes[:, :16], qv.scales, 32), lambda: F.MXFP4(qv.codes, qv.scales, 65), lambda: F.MXFP4(qv.codes[1:], qv.scales, 64),
+                 lambda: F.masked_linear_mxfp4_backward(x, qv, qt, mask),
+                 lambda: F.MaskedLinearMXFP4.apply(x.clone().requires_grad_(), qv, qt, mask)):  # 32 output features: no backward for them
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        F.MaskedLinearMXFP4.apply(x, qv, weight(32, 64, 1), mask)
+
+
+# ---- the feed-forward layer -----------------------------------------------------------------------------------------------------
+
+def ffn_case(m, d, h, kind, seed=11):
+    w = {n: weight(d, h, seed + i, 1.2 / h ** 0.5) if n[1] == "2" else weight(h, d, seed + i, 1.2 / d ** 0.5) for i, n in enumerate(FFN)}
+    x = rows(m, d, seed + 9)
+    return x, [F.mxfp4_quantise(w[n]) for n in FFN], a_mask(m, kind, seed), ref.values(x), {n: ref.values(w[n]) for n in FFN}
+
+
+@pytest.mark.parametrize("kind", ["mixed", "visual", "text"])
+@pytest.mark.parametrize("m,d,h", [(1, 32, 32), (1, 1024, 2048), (2, 40, 33), (5, 512, 520), (16, 256, 1000), (17, 1000, 1056), (31, 1032, 2000), (48, 544, 96), (64, 768, 1544),
+                                   (64, 31, 65), (65, 64, 40), (66, 33, 31), (100, 512, 1032), (129, 520, 776), (300, 1024, 2816), (515, 264, 520)])
+def test_ffn_forward(m, d, h, kind):
+    note(f"ffn {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    value, bound = ref.ffn(a, w, mask)
+    y = F.MaskedFFNMXFP4.apply(x, *q, mask)
+    within(y, value, bound, "rows in bf16")
+    within(F.masked_ffn_mxfp4_forward(F.mxfp4_quantise(x), *q, mask), value, bound, "rows in MXFP4")
+    assert torch.equal(y, F.MaskedFFNMXFP4.apply(x, *q, mask)), "the same call twice"
+
+
+@pytest.mark.parametrize("m,d,h,kind", [(2100, 512, 4160, "mixed"), (3000, 264, 4104, "visual"), (4500, 1024, 2080, "mixed")])
+def test_ffn_forward_on_large_tiles(m, d, h, kind):
+    note(f"ffn large {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    value, bound = ref.ffn(a, w, mask)
+    within(F.masked_ffn_mxfp4_forward(x, *q, mask), value, bound, "rows in bf16")
+    y, pre = F.masked_ffn_mxfp4_forward(x, *q, mask, save_pre=True)
+    within(y, value, bound, "with the projections kept")
+
+
+@pytest.mark.parametrize("m", [7, 64, 65, 200])
+def test_ffn_keeps_its_projections_in_routed_order(m):
+    note(f"ffn pre {m}")
+    d, h = 96, 136
+    x, q, mask, a, w = ffn_case(m, d, h, "mixed")
+    y, pre = F.masked_ffn_mxfp4_forward(x, *q, mask, save_pre=True)
+    order = torch.cat((mask.nonzero().view(-1), (~mask).nonzero().view(-1)))
+    for half, names in ((0, ("w1", "u1")), (h, ("w3", "u3"))):
+        value, bound = ref.linear(a, w[names[0]], w[names[1]], mask)
+        within(pre[:, half:half + h], value[order], bound[order], f"projection at {half}")
+    within(y, *ref.ffn(a, w, mask), "result")
+
+
+def test_ffn_infinities_stay_in_their_rows():
+    note("ffn inf")
+    for m in (6, 90):
+        x, q, mask, _, w = ffn_case(m, 256, 320, "mixed")
+        x[2, 17] = float("inf")
+        value, bound = ref.ffn(ref.values(x).nan_to_num(0.0), w, mask)
+        value[2] = float("nan")
+        within(F.masked_ffn_mxfp4_forward(x, *q, mask), value, bound, "row 2 is NaN, the others not")
+
+
+# ---- gradients ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["mixed", "visual", "text"])
+@pytest.mark.parametrize("m,k,n", [(1, 8, 64), (5, 264, 128), (64, 512, 136), (65, 32, 64), (100, 1032, 200), (300, 256, 520), (2050, 1024, 1024)])
+def test_linear_gradient(m, k, n, kind):
+    note(f"linear grad {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    g = rows(m, n, 3)
+    x.requires_grad_()
+    y = F.MaskedLinearMXFP4.apply(x, qv, qt, mask)
+    within(y.detach(), *ref.linear(a, wv, wt, mask), "forward")
+    da, = torch.autograd.grad(y, x, g)
+    value, bound = ref.linear_grad(g.double(), wv, wt, mask)
+    within(da, value, bound, "gradient")
+    wide = torch.empty(m, n + 3, device="cuda", dtype=torch.bfloat16)
+    wide[:, 1:n + 1] = g
+    within(F.masked_linear_mxfp4_backward(wide[:, 1:n + 1], qv, qt, mask), value, bound, "an upstream gradient off 16 bytes")
+
+
+@pytest.mark.parametrize("kind", ["mixed", "visual", "text"])
+@pytest.mark.parametrize("m,d,h", [(1, 64, 64), (7, 136, 72), (64, 256, 520), (65, 128, 200), (130, 264, 512), (300, 512, 1032), (1100, 1024, 2056)])
+def test_ffn_gradient(m, d, h, kind):
+    note(f"ffn grad {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    g = rows(m, d, 3)
+    x.requires_grad_()
+    y = F.MaskedFFNMXFP4.apply(x, *q, mask)
+    within(y.detach(), *ref.ffn(a, w, mask), "forward")
+    da, = torch.autograd.grad(y, x, g)
+    within(da, *ref.ffn_grad(g, a, w, mask), "gradient")
+    with torch.no_grad():
+        assert not F.MaskedFFNMXFP4.apply(x, *q, mask).requires_grad
+
+
+def test_rows_in_mxfp4_carry_no_gradient():
+    note("no gradient")
+    x, q, mask, _, _ = ffn_case(70, 64, 64, "mixed")
+    y = F.MaskedFFNMXFP4.apply(F.mxfp4_quantise(x.requires_grad_()), *q, mask)
+    assert not y.requires_grad
+
+
+# ---- a run of them together, as a block uses them --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("batch,seq", [(1, 1), (3, 9), (2, 150)])
+def test_modules_of_a_block(batch, seq):
+    note(f"modules {batch}x{seq}")
+    torch.manual_seed(4)
+    d, h = 256, 520
+    proj, ffn = F.MaskedLinearModule(d, d, device="cuda"), F.MaskedFFNModule(d, h, device="cuda")
+    proj4, ffn4 = F.MaskedLinearMXFP4Module.from_module(proj), F.MaskedFFNMXFP4Module.from_module(ffn)
+    x = rows(batch * seq, d, 6).view(batch, seq, d).requires_grad_()
+    mask = a_mask(batch * seq, "mixed").view(batch, seq)
+    y = ffn4(proj4(x, mask), mask)
+    y.backward(torch.ones_like(y))
+    m, a = mask.view(-1), ref.values(x.detach().view(-1, d))
+    mid = proj4(x, mask).detach().view(-1, d)
+    within(mid, *ref.linear(a, ref.values(proj.linear_v.weight.detach()), ref.values(proj.linear_t.weight.detach()), m), "projection")
+    w = {n: ref.values(getattr(ffn, n).weight.detach()) for n in FFN}
+    within(y.detach().view(-1, d), *ref.ffn(ref.values(mid), w, m), "feed-forward")
+    assert x.grad.isfinite().all() and x.grad.abs().max() > 0
+    # a state that is saved and loaded, copied and moved answers alike
+    fresh = F.MaskedFFNMXFP4Module(d, h, device="cuda")
+    fresh.load_state_dict(ffn4.state_dict())
+    moved = copy.deepcopy(ffn4).cpu().cuda()
+    with torch.no_grad():
+        for other in (fresh, moved, copy.deepcopy(ffn4)):
+            assert torch.equal(other(proj4(x, mask), mask), y)
+
+
+def test_rows_quantised_once_serve_several_projections():
+    note("shared rows")
+    x, qv, qt, mask, _ = linear_case(200, 512, 96, "mixed")
+    q = F.mxfp4_quantise(x)
+    routing = F.route(mask)
+    for seed in (3, 5):
+        a, b = F.mxfp4_quantise(weight(96, 512, seed)), F.mxfp4_quantise(weight(96, 512, seed + 1))
+        assert torch.equal(F.masked_linear_mxfp4_forward(q, a, b, mask, routing=routing), F.masked_linear_mxfp4_forward(x, a, b, mask))
+
+
+@pytest.mark.parametrize("m", [4, 64, 150, 2100])
+def test_graphs_and_streams(m):
+    note(f"graph {m}")
+    d, h = 256, 4160 if m > 1000 else 544
+    x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+    p = F.mxfp4_quantise(weight(d, d, 2)), F.mxfp4_quantise(weight(d, d, 3))
+
+    def block(t):
+        with torch.no_grad():
+            return F.MaskedFFNMXFP4.apply(F.MaskedLinearMXFP4.apply(t, *p, mask), *q, mask)
+
+    want = block(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(block(x), want)
+    torch.cuda.current_stream().wait_stream(side)
+    held = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = block(held)
+    for seed in (21, 22, 23):
+        held.copy_(rows(m, d, seed))
+        graph.replay()
+        replayed = out.clone()
+        eager = block(held)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, eager)

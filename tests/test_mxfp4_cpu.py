@@ -1,0 +1,149 @@
+"""MXFP4 without a GPU: the oracle's rounding against the format's own definition, its gradients against differences, what the
+operators refuse, and the C ABI's answers to bad arguments."""
+import ctypes
+
+import pytest
+import torch
+
+import ffn_kernel_amd as F
+from ffn_kernel_amd import _lib
+from oracle import mxfp4 as ref
+
+
+def test_oracle_rounds_to_the_nearest_with_ties_to_even_codes():
+    # block maximum 4: scale 1
+    t = torch.zeros(1, 32)
+    given = [4.0, 0.25, 0.26, 0.75, 0.74, 1.25, 1.75, 2.5, 3.5, 3.49, -0.25, -0.75, -2.5, -3.5, -1.3]
+    wanted = [4.0, 0.0, 0.5, 1.0, 0.5, 1.0, 2.0, 2.0, 4.0, 3.0, 0.0, -1.0, -2.0, -4.0, -1.5]
+    t[0, :len(given)] = torch.tensor(given)
+    assert ref.values(t)[0, :len(given)].tolist() == wanted
+    assert ref.exponents(t).item() == 0
+    t[0, 0] = 5.0   # a tie between 4 and 6: 4 has the even code
+    assert ref.values(t)[0, 0].item() == 4.0
+    t[0, 0] = 7.99  # the largest of a block saturates
+    assert ref.values(t)[0, 0].item() == 6.0
+    t[0, 0] = 8.0
+    assert ref.exponents(t).item() == 1 and ref.values(t)[0, 0].item() == 8.0
+
+
+def test_oracle_blocks_and_extremes():
+    t = torch.zeros(3, 70)
+    t[0, 40], t[0, 69] = 3.0, -1.0
+    t[1, 3], t[1, 35] = float("inf"), float("nan")
+    t[2, 0] = 2.0 ** -140
+    v = ref.values(t)
+    assert v.shape == (3, 70) and v[0, 40].item() == 3.0 and v[0, 69].item() == -1.0
+    assert ref.exponents(t)[0].tolist() == [-127, -1, -2]
+    assert v[1, :64].isnan().all() and not v[1, 64:].isnan().any()
+    assert v[2].abs().max().item() == 0.0  # far under the smallest scale
+    codes, scales = ref.pack(t)
+    assert codes.shape == (3, 48) and scales.tolist()[0] == [0, 126, 125] and scales[1, 0].item() == 255
+    assert codes[0, 20].item() == 7 and codes[0, 34].item() == 14 << 4  # column 40 in a low half, 69 in a high one
+
+
+def test_doubtful_covers_both_sides_of_a_border():
+    h = torch.zeros(1, 32, dtype=torch.float64)
+    h[0, 0], h[0, 1], h[0, 2] = 4.0 + 1e-3, 2.5, 1.3
+    bound = torch.full_like(h, 1e-6)
+    d = ref.doubtful(h, bound)
+    assert d[0, 1].item() == 1.0 and d[0, 2].item() == 0.0 and d[0, 0].item() == 0.0
+    h[0, 0] = 8.0  # the scale itself is in doubt: 1 or 2
+    assert ref.doubtful(h, bound)[0, 0].item() >= 2.0
+
+
+# The rows' gradient is that of the function with both quantisations passed over, at the quantised rows.
+def test_oracle_gradients_against_differences():
+    gen = torch.Generator().manual_seed(3)
+    M, d, h = 5, 64, 96
+    draw = lambda *s: ref.values(torch.randn(*s, generator=gen))
+    a, mask = draw(M, d), torch.tensor([True, False, True, True, False])
+    w = {n: draw(d, h) if n[1] == "2" else draw(h, d) for n in ("w1", "w2", "w3", "u1", "u2", "u3")}
+    g = torch.randn(M, d, generator=gen, dtype=torch.float64)
+
+    def loss(x):
+        rows = []
+        for s, on in (("w", mask), ("u", ~mask)):
+            y = torch.nn.functional.silu(x @ w[s + "1"].T) * (x @ w[s + "3"].T) @ w[s + "2"].T
+            rows.append((y * g * on.unsqueeze(-1)).sum())
+        return sum(rows)
+
+    da, _ = ref.ffn_grad(g, a, w, mask)
+    for _ in range(6):
+        v = torch.randn(M, d, generator=gen, dtype=torch.float64)
+        eps = 1e-6
+        slope = (loss(a + eps * v) - loss(a - eps * v)) / (2 * eps)
+        assert abs(slope - (da * v).sum()) <= 1e-6 * (da.abs() * v.abs()).sum()
+    gl = torch.randn(M, h, generator=gen, dtype=torch.float64)
+    dl, _ = ref.linear_grad(gl, w["w1"], w["u1"], mask)
+    v = torch.randn(M, d, generator=gen, dtype=torch.float64)
+    c = torch.where(mask.unsqueeze(-1), v @ w["w1"].T, v @ w["u1"].T)
+    assert abs((c * gl).sum() - (dl * v).sum()) <= 1e-9 * (dl.abs() * v.abs()).sum()
+
+
+@pytest.mark.parametrize("call", [
+    lambda: F.mxfp4_quantise([1.0]),
+    lambda: F.mxfp4_dequantise(torch.zeros(2, 2)),
+    lambda: F.masked_linear_mxfp4_forward(F, None, None, None),
+])
+def test_wrong_kinds_are_type_errors(call):
+    with pytest.raises(TypeError):
+        call()
+
+
+@pytest.mark.parametrize("t", [torch.zeros(4), torch.zeros(2, 2, dtype=torch.float64), torch.zeros(2, 2, dtype=torch.int8), torch.zeros(2, 32)])
+def test_quantise_refuses(t):
+    with pytest.raises(ValueError):
+        F.mxfp4_quantise(t)
+
+
+def test_from_parts_refuses():
+    codes, scales = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)
+    for c, s, k in ((codes, scales, 64), (codes, scales[:3], 32), (codes.float(), scales, 32), (codes[0], scales, 32), (codes, scales, -1),
+                    (codes, scales[:, :0], 32)):
+        with pytest.raises((ValueError, RuntimeError)):
+            F.MXFP4.from_parts(c, s, k)
+    with pytest.raises(ValueError, match="GPU"):
+        F.MXFP4.from_parts(codes, scales, 32)  # all there, but in host memory
+
+
+def test_workspace_and_refusals_of_the_c_abi():
+    lib = _lib.load()
+    bad = ctypes.c_size_t(-1).value
+    size = lib.ffnk_mxfp4_workspace_bytes
+    assert size(_lib.OP_LINEAR_FWD, 8, 4096, 4096) >= 8 * 4096 * 17 // 32
+    assert size(_lib.OP_FFN_FWD, 300, 4096, 14336) >= 300 * (4096 + 14336) * 17 // 32 + 300 * 4
+    assert size(_lib.OP_FFN_BWD, 300, 4096, 14336) >= 6 * 4096 * 14336 * 2
+    assert size(_lib.OP_LINEAR_BWD, 300, 512, 256) >= 2 * 512 * 256 * 2
+    assert size(_lib.OP_FFN_UP, 300, 512, 256) == bad and size(_lib.OP_LINEAR_FWD, -1, 8, 8) == bad and size(_lib.OP_LINEAR_FWD, 8, 0, 8) == bad
+    t = _lib.Mxfp4Struct(0x1000, 0x2000)
+    q, half, off = ctypes.addressof(t), _lib.Mxfp4Struct(0x1000, None), _lib.Mxfp4Struct(0x1008, 0x2000)
+    E = dict(NULL=-1, SHAPE=-2, STRIDE=-3, ALIGN=-4, WORKSPACE=-5, OP=-6)
+    quantise, dequantise, linear, ffn = lib.ffnk_mxfp4_quantise, lib.ffnk_mxfp4_dequantise, lib.ffnk_mxfp4_linear_fwd, lib.ffnk_mxfp4_ffn_fwd
+    assert quantise(0x100, 0, 32, q, -1, 32, None) == E["SHAPE"]
+    assert quantise(0x100, 7, 32, q, 1, 32, None) == E["OP"]
+    assert quantise(None, 0, 32, q, 1, 32, None) == E["NULL"]
+    assert quantise(0x100, 0, 31, q, 1, 32, None) == E["STRIDE"]
+    assert quantise(0x101, 0, 32, q, 1, 32, None) == E["ALIGN"] and quantise(0x102, 2, 32, q, 1, 32, None) == E["ALIGN"]
+    assert quantise(0x100, 0, 32, ctypes.addressof(half), 1, 32, None) == E["NULL"]
+    assert quantise(0x100, 0, 32, ctypes.addressof(off), 1, 32, None) == E["ALIGN"]
+    assert quantise(None, 0, 0, None, 0, 32, None) == 0
+    assert dequantise(q, None, 0, 32, 1, 32, None) == E["NULL"] and dequantise(q, 0x100, 0, 8, 1, 32, None) == E["STRIDE"]
+    ws = (0x4000, 1 << 30)
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, None, 0, None, None) == E["WORKSPACE"]
+    assert linear(0x100, 64, q, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]      # x and xq
+    assert linear(None, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert linear(0x100, 64, None, q, None, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert linear(0x100, 64, None, q, q, None, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert linear(0x100, 63, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["STRIDE"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 63, 4, 64, 64, *ws, None, None) == E["STRIDE"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 0, 64, *ws, None, None) == E["SHAPE"]
+    assert linear(None, 0, q, q, q, 0x10, 0x100, 64, 1 << 24, 1 << 10, 64, 0x4000, 1 << 62, None, None) == E["SHAPE"]  # past 32-bit offsets
+    assert ffn(0x100, 64, None, q, q, q, q, q, None, 0x10, 0x100, 64, None, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert b"U3" in lib.ffnk_last_error()
+    lb, fb = lib.ffnk_mxfp4_linear_bwd, lib.ffnk_mxfp4_ffn_bwd
+    assert lb(0x100, 64, q, q, 0x10, 0x100, 63, 4, 63, 64, *ws, None, None) == E["STRIDE"]
+    assert lb(0x100, 72, q, q, 0x10, 0x100, 64, 4, 64, 72, *ws, None, None) == E["STRIDE"]
+    assert lb(0x100, 64, q, q, 0x10, 0x100, 64, 4, 64, 64, 0x4000, 64, None, None) == E["WORKSPACE"]
+    assert fb(0x100, 64, q, q, q, q, q, q, 0x10, None, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert fb(0x100, 64, q, q, q, q, q, q, 0x10, 0x108, 0x100, 64, 4, 64, 64, *ws, None, None) == E["STRIDE"]
+    assert linear(None, 0, None, None, None, None, None, 64, 0, 64, 64, None, 0, None, None) == 0  # no rows
