@@ -93,25 +93,24 @@ __device__ __forceinline__ void mx_mainloop(const MxGemmArgs& g, const TileCoord
     scale_base[s] = wave_uniform(scale_base[s]);
   }
 
-  auto load = [&](int kt) {
-    uint8_t* stage = lds + (kt & 1) * Cfg::STAGE_BYTES;
-    const uint32_t back = kt == nk - 1 ? last_back : 0u;
-#pragma unroll
-    for (int j = 0; j < NJA; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, FFNK_LDS_PTR(stage + (j * NW + wave) * 1024), 16, off_a[j] + back, kt * kRowBytes, 0, 0);
-#pragma unroll
-    for (int j = 0; j < NJB; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB[Cfg::DUAL && j >= NJB / 2], FFNK_LDS_PTR(stage + Cfg::A_BYTES + (j * NW + wave) * 1024), 16,
-                                               off_b[j] + back, kt * kRowBytes, 0, 0);
-    if ((kt & 1) == 0) {
-      uint8_t* scales = lds + 2 * Cfg::STAGE_BYTES + ((kt >> 1) & 1) * Cfg::SCALE_BYTES;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int q = s * NW + wave;
-        if (NG % NW == 0 || q < NG)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scale_base[s]), 0, 0xffffffff, 0x00020000),
-                                                   FFNK_LDS_PTR(scales + q * 1024), 16, off_s[s], (kt >> 1) * 16, 0, 0);
-      }
+  // Load l of stage kt (of parity u): weight rows, token rows, then - with the first of two stages - their scales.
+  constexpr int LOADS = NJA + NJB;
+  auto load = [&](int l, int u, int kt) {
+    uint8_t* stage = lds + u * Cfg::STAGE_BYTES;
+    if (l < LOADS) {
+      const uint32_t back = kt == nk - 1 ? last_back : 0u;
+      const int j = l < NJB ? l : l - NJB;
+      if (l < NJB)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB[Cfg::DUAL && j >= NJB / 2], FFNK_LDS_PTR(stage + Cfg::A_BYTES + (j * NW + wave) * 1024), 16,
+                                                 off_b[j] + back, kt * kRowBytes, 0, 0);
+      else
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, FFNK_LDS_PTR(stage + (j * NW + wave) * 1024), 16, off_a[j] + back, kt * kRowBytes, 0, 0);
+    } else {
+      const int s = l - LOADS, q = s * NW + wave;
+      if (NG % NW == 0 || q < NG)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(scale_base[s]), 0, 0xffffffff, 0x00020000),
+            FFNK_LDS_PTR(lds + 2 * Cfg::STAGE_BYTES + ((kt >> 1) & 1) * Cfg::SCALE_BYTES + q * 1024), 16, off_s[s], (kt >> 1) * 16, 0, 0);
     }
   };
 
@@ -119,36 +118,95 @@ __device__ __forceinline__ void mx_mainloop(const MxGemmArgs& g, const TileCoord
 #pragma unroll
   for (int s = 0; s < 4; ++s) koff[s] = lds_swizzle(tl.lr, 4 * tl.lh + s);
   const uint32_t a_base = (uint32_t)(tl.wm * Cfg::WTM) * kRowBytes;
+  i32x4_t fa[2][TM], fb[2][TN];
+  int sa[2][TM], sb[2][TN];
+  // Fragment f of step s of a stage of parity u: token rows, then weight rows; their scales.
+  auto read = [&](int f, int u, int s) {
+    const uint8_t* stage = lds + u * Cfg::STAGE_BYTES;
+    if (f < TN) fb[s & 1][f] = *reinterpret_cast<const i32x4_t*>(stage + Cfg::A_BYTES + b_frag_row<Cfg>(tl.wn, f) * kRowBytes + koff[s]);
+    else fa[s & 1][f - TN] = *reinterpret_cast<const i32x4_t*>(stage + a_base + (f - TN) * 32 * kRowBytes + koff[s]);
+  };
+  auto read_scale = [&](int f, int u, int kt) {
+    const uint8_t* scales = lds + 2 * Cfg::STAGE_BYTES + ((kt >> 1) & 1) * Cfg::SCALE_BYTES + 8 * u + 4 * tl.lh;
+    if (f < TN) sb[u][f] = *reinterpret_cast<const int*>(scales + (BM + b_frag_row<Cfg>(tl.wn, f) + tl.lr) * 16);
+    else sa[u][f - TN] = *reinterpret_cast<const int*>(scales + (tl.wm * Cfg::WTM + (f - TN) * 32 + tl.lr) * 16);
+  };
 
-  zero_acc<Cfg>(acc);
-  load(kt0);
-  for (int kt = kt0; kt < kt1; ++kt) {
-    dma_wait_barrier<0>();  // stage kt has landed, and every wave has read the last of stage kt - 1
-    if (kt + 1 < kt1) load(kt + 1);
-    const uint8_t* stage = lds + (kt & 1) * Cfg::STAGE_BYTES;
-    const uint8_t* scales = lds + 2 * Cfg::STAGE_BYTES + ((kt >> 1) & 1) * Cfg::SCALE_BYTES + 8 * (kt & 1) + 4 * tl.lh;
-    int sa[TM], sb[TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) sa[i] = *reinterpret_cast<const int*>(scales + (tl.wm * Cfg::WTM + i * 32 + tl.lr) * 16);
-#pragma unroll
-    for (int j = 0; j < TN; ++j) sb[j] = *reinterpret_cast<const int*>(scales + (BM + b_frag_row<Cfg>(tl.wn, j) + tl.lr) * 16);
-    i32x4_t fa[2][TM], fb[2][TN];
-    auto read = [&](int s) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-        fb[s & 1][j] = *reinterpret_cast<const i32x4_t*>(stage + Cfg::A_BYTES + b_frag_row<Cfg>(tl.wn, j) * kRowBytes + koff[s]);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) fa[s & 1][i] = *reinterpret_cast<const i32x4_t*>(stage + a_base + i * 32 * kRowBytes + koff[s]);
-    };
-    read(0);
+  // A stage is four steps of 64 columns, TM x TN matrix instructions each.  Behind them, spread over the step, the next step's
+  // fragments are read (the last step's early, the next stage's first ones behind the data barrier).  Two barriers a stage:
+  //   RELEASE: every wave has read the last of this stage - the loads of the stage after next go into its memory from here on
+  //   DATA: the next stage has landed
+  // which leaves the loads 1.2 to 1.5 stages to land.
+  constexpr int NM = TM * TN, NF = TM + TN, LEV = NM >= 16 ? 2 : 1;
+  constexpr int RELEASE = 3 * NM - (NM >= 16 ? 4 : 1), DATA = 3 * NM + (NM >= 16 ? 6 : 1), TURN = 4 * NM;
+  constexpr int FIRST = (TURN - RELEASE) / LEV, BEFORE = (DATA - RELEASE) / LEV;  // loads behind RELEASE in this stage, and of these ahead of DATA
+  static_assert(FIRST <= LOADS && LOADS + NS - FIRST <= RELEASE / LEV, "the loads of a stage go out between its two RELEASE barriers");
+  static_assert(NG % NW == 0, "every wave issues as many loads, which it counts");
+  auto stage = [&](auto parity, int kt, auto next_, auto next2_) {
+    constexpr int u = decltype(parity)::value;
+    const bool next = next_, next2 = next2_;         // stages kt + 1 and kt + 2 are there
+    constexpr int ALL1 = LOADS + (u == 1 ? NS : 0);  // loads of stage kt + 1 (of the other parity)
     static_for<0, 4>([&](auto step) {
       constexpr int s = decltype(step)::value;
-      if (s < 3) read(s + 1);
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int m = 0; m < NM; ++m) {
+        const int t = s * NM + m;
+        if (t == RELEASE && next2) dma_wait_barrier<63>();
+        if (t == DATA && next) {
+          if (next2) dma_wait_barrier<BEFORE>();
+          else dma_wait_barrier<0>();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const int i = m / TN, j = m % TN;
+        acc[i][j] = mx_mfma32<s>(fb[s & 1][j], fa[s & 1][i], acc[i][j], sb[u][j], sa[u][i]);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mx_mfma32<s>(fb[s & 1][j], fa[s & 1][i], acc[i][j], sb[j], sa[i]);
+        for (int f = 0; f < NF; ++f) {
+          if (s < 3 ? f * (s == 2 ? NM / 2 : NM) / NF == m : DATA + f * (TURN - DATA) / NF == t && next) {
+            if (s < 3) {
+              read(f, u, s + 1);
+            } else {
+              read_scale(f, u ^ 1, kt + 1);
+              read(f, u ^ 1, 0);
+            }
+          }
+        }
+        if (t >= RELEASE) {
+          if ((t - RELEASE) % LEV == LEV - 1 && next2) load((t - RELEASE) / LEV, u, kt + 2);
+        } else if (t % LEV == LEV - 1 && FIRST + t / LEV < ALL1 && next) {
+          load(FIRST + t / LEV, u ^ 1, kt + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     });
+  };
+
+  zero_acc<Cfg>(acc);
+#pragma unroll
+  for (int l = 0; l < LOADS + NS; ++l) load(l, 0, kt0);
+  if (kt0 + 1 < kt1) {
+#pragma unroll
+    for (int l = 0; l < FIRST; ++l) load(l, 1, kt0 + 1);
+    dma_wait_barrier<FIRST>();
+  } else {
+    dma_wait_barrier<0>();
+  }
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    read_scale(f, 0, kt0);
+    read(f, 0, 0);
+  }
+  constexpr auto even = std::integral_constant<int, 0>{};
+  constexpr auto odd = std::integral_constant<int, 1>{};
+  constexpr auto yes = std::true_type{};
+  int kt = kt0;
+  for (; kt + 3 < kt1; kt += 2) {  // no branches inside
+    stage(even, kt, yes, yes);
+    stage(odd, kt + 1, yes, yes);
+  }
+  for (; kt < kt1; kt += 2) {
+    stage(even, kt, kt + 1 < kt1, kt + 2 < kt1);
+    if (kt + 1 < kt1) stage(odd, kt + 1, kt + 2 < kt1, kt + 3 < kt1);
   }
 #endif
 }
