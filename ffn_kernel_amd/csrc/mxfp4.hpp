@@ -18,24 +18,61 @@ __host__ __device__ constexpr int64_t mx_blocks(int64_t columns) { return cdiv64
 __host__ __device__ constexpr int64_t mx_code_stride(int64_t columns) { return mx_blocks(columns) * 16; }
 __host__ __device__ constexpr int64_t mx_scale_stride(int64_t columns) { return round_up64(mx_blocks(columns), 16); }
 
-// Scale byte of a block whose largest magnitude is `top` (its fp32 bits without the sign): the largest power of two not above it
-// over 4, the largest power of two of the numbers, so that the largest one lands in [4, 8) and saturates at 6.  Blocks with an
-// infinity or a NaN are NaN as a whole.
-__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
-  const uint32_t e = top >> 23;
+// Scale byte of a block whose largest magnitude is `top`: the largest power of two not above it over 4, the largest power of two of
+// the numbers, so that the largest one lands in [4, 8) and saturates at 6.  Blocks with an infinity or a NaN are NaN as a whole.
+__device__ __forceinline__ uint32_t mx_scale_byte(float top) {
+  const uint32_t e = __builtin_bit_cast(uint32_t, top) >> 23;
   return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
 }
-// 2^(127 - byte): every block's values are brought to the numbers' range by an exact product.
-__device__ __forceinline__ float mx_inverse(uint32_t byte) { return __builtin_bit_cast(float, (byte == 255 ? 127u : 254u - byte) << 23); }
 __device__ __forceinline__ float mx_scale(uint32_t byte) {
   return __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
 }
 
-// Codes of four scaled values in the low 16 bits, rounded to the nearest number (ties to the even code), saturated.
-__device__ __forceinline__ uint32_t mx_codes4(float a, float b, float c, float d) {
+// The largest of `top` and the magnitudes of a and b; a NaN if one of them is.
+__device__ __forceinline__ float mx_top(float top, float a, float b) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  uint32_t v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, 1.0f, 0);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, c, d, 1.0f, 1);
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(a), __builtin_fabsf(b)), top);
+#else
+  return top;
+#endif
+}
+
+// Lane l exchanges with lane l + 32 (16: with lane l + 16 of its half).
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+__device__ __forceinline__ u32x2_t lane_swap32(uint32_t a, uint32_t b) {  // {a, a of lane + 32} below, {b of lane - 32, b} above
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+#else
+  return u32x2_t{a, b};
+#endif
+}
+__device__ __forceinline__ u32x2_t lane_swap16(uint32_t a, uint32_t b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+#else
+  return u32x2_t{a, b};
+#endif
+}
+__device__ __forceinline__ float mx_top_of(u32x2_t v) {
+  const uint32_t a = v[0], b = v[1];  // (a bit cast of an element as such reads the first one)
+  return mx_top(0.f, __builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float mx_top_across32(float top) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+  return mx_top_of(lane_swap32(bits, bits));
+}
+__device__ __forceinline__ float mx_top_across16(float top) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, top);
+  return mx_top_of(lane_swap16(bits, bits));
+}
+
+// Codes of four values of a block in the low 16 bits: divided by its scale (the instruction takes the exponent of its operand,
+// which for byte 0 is that of 2^-127 as well), rounded to the nearest number, ties to the even code, saturated.
+__device__ __forceinline__ uint32_t mx_codes4(float a, float b, float c, float d, uint32_t byte) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const float scale = __builtin_bit_cast(float, byte << 23);
+  const uint32_t v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, a, b, scale, 0);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, c, d, scale, 1);
 #else
   return 0;
 #endif

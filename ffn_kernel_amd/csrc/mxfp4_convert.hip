@@ -66,6 +66,15 @@ __device__ __forceinline__ ItemAt item_at(const ItemShape& s, uint32_t block, in
   return {r < s.rows_per_wg ? (int)block * s.rows_per_wg + r : 0x7fffffff, j - r * s.runs};
 }
 
+template <int PATTERN>
+__device__ __forceinline__ float quad_lane(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), PATTERN, 0xf, 0xf, true));
+#else
+  return v;
+#endif
+}
+
 // U items of a lane, their loads in flight together.  VEC: rows are whole, aligned 16-byte pieces.
 template <int TYPE, int U, bool VEC>
 __global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a, const ItemShape shape, const int nb) {
@@ -93,24 +102,18 @@ __global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a
   const int64_t ldc = (int64_t)nb * 16, lds = round_up64(nb, 16);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float f[kItem];
-    uint32_t top = 0;
+    float f[kItem], top = 0.f;
 #pragma unroll
-    for (int e = 0; e < kItem; ++e) {
-      f[e] = E::load(v[u].v[e]);
-      const uint32_t bits = __builtin_bit_cast(uint32_t, f[e]) & 0x7fffffffu;
-      top = bits > top ? bits : top;
-    }
+    for (int e = 0; e < kItem; ++e) f[e] = E::load(v[u].v[e]);
+#pragma unroll
+    for (int e = 0; e < kItem; e += 2) top = mx_top(top, f[e], f[e + 1]);
     // the quad's largest (a quad's items are one block: runs is a multiple of 4, and so is every workgroup's first item)
-    uint32_t other = (uint32_t)__shfl_xor((int)top, 1);
-    top = other > top ? other : top;
-    other = (uint32_t)__shfl_xor((int)top, 2);
-    top = other > top ? other : top;
+    top = mx_top(top, quad_lane<0xb1>(top), quad_lane<0x4e>(top));  // lanes 1 0 3 2, lanes 2 3 0 1
+    top = mx_top(top, quad_lane<0xb1>(top), 0.f);
     const uint32_t byte = mx_scale_byte(top);
-    const float inv = mx_inverse(byte);
     if (at[u].row >= a.rows || at[u].run >= 4 * nb) continue;
-    const uint32_t lo = mx_codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-    const uint32_t hi = mx_codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
+    const uint32_t lo = mx_codes4(f[0], f[1], f[2], f[3], byte);
+    const uint32_t hi = mx_codes4(f[4], f[5], f[6], f[7], byte);
     *reinterpret_cast<uint32_t*>(a.codes + at[u].row * ldc + at[u].run * 4) = lo | (hi << 16);
     if ((at[u].run & 3) == 0) {
       const int b = at[u].run >> 2;
@@ -145,9 +148,9 @@ __global__ __launch_bounds__(256) void mx_dequantise_kernel(const MxDequantiseAr
   for (int u = 0; u < U; ++u) {
     const int column = at[u].run * kItem;
     if (at[u].row >= a.rows || column >= a.columns) continue;
-    const float scale = mx_scale(byte[u]);
     Run<T> v;
 #if defined(__HIP_DEVICE_COMPILE__)
+    const float scale = mx_scale(byte[u]);
 #define FFNK_MX_PAIR(I)                                                              \
   {                                                                                  \
     const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[u], 1.0f, I);      \

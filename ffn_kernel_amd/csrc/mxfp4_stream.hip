@@ -111,26 +111,19 @@ __global__ __launch_bounds__(WAVES * kWave) void mx_stream_kernel(const MxStream
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (t * 16 >= rows) continue;
-      float h[8];
-      uint32_t top = 0;
+      float h[8], top = 0.f;
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
         h[v] = swiglu(acc[v / 4][t][v % 4], acc[TILES + v / 4][t][v % 4]);
         if (n0 + v / 4 * 16 + lg * 4 + v % 4 >= a.N) h[v] = 0.f;
-        const uint32_t bits = __builtin_bit_cast(uint32_t, h[v]) & 0x7fffffffu;
-        top = bits > top ? bits : top;
       }
 #pragma unroll
-      for (int far = 16; far <= 32; far *= 2) {
-        const uint32_t other = (uint32_t)__shfl_xor((int)top, far);
-        top = other > top ? other : top;
-      }
-      const uint32_t byte = mx_scale_byte(top);
-      const float inv = mx_inverse(byte);
+      for (int v = 0; v < 8; v += 2) top = mx_top(top, h[v], h[v + 1]);
+      const uint32_t byte = mx_scale_byte(mx_top_across32(mx_top_across16(top)));
       if (t * 16 + lr >= rows) continue;
       uint8_t* hc = a.H + token[t] * ldh + b * 16 + lg * 2;
-      *reinterpret_cast<uint16_t*>(hc) = (uint16_t)mx_codes4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-      *reinterpret_cast<uint16_t*>(hc + 8) = (uint16_t)mx_codes4(h[4] * inv, h[5] * inv, h[6] * inv, h[7] * inv);
+      *reinterpret_cast<uint16_t*>(hc) = (uint16_t)mx_codes4(h[0], h[1], h[2], h[3], byte);
+      *reinterpret_cast<uint16_t*>(hc + 8) = (uint16_t)mx_codes4(h[4], h[5], h[6], h[7], byte);
       if (lg == 0) {
         uint8_t* hs = a.SH + token[t] * ldsh;
         hs[b] = (uint8_t)byte;
