@@ -99,10 +99,10 @@ _SIGNATURES.update({
     "ffnk_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "ffnk_mxfp4_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,  # x, xq, Wv, Wt, mask
                                       c_void_p, c_int64, c_int64, c_int64, c_int64,               # y, M, K, N
-                                      c_void_p, c_size_t, c_void_p, c_void_p]),
+                                      c_void_p, c_size_t, c_void_p, c_void_p, c_int]),            # ... routing, made
     "ffnk_mxfp4_ffn_fwd": (c_int, [c_void_p, c_int64, c_void_p] + [c_void_p] * 6 + [c_void_p,     # x, xq, weights, mask
                                    c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,        # out, pre, M, d, h
-                                   c_void_p, c_size_t, c_void_p, c_void_p]),
+                                   c_void_p, c_size_t, c_void_p, c_void_p, c_int]),
     "ffnk_mxfp4_linear_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p,            # g, Wv, Wt, mask
                                       c_void_p, c_int64, c_int64, c_int64, c_int64,               # dx, M, K, N
                                       c_void_p, c_size_t, c_void_p, c_void_p]),

@@ -9,6 +9,7 @@
 #include <Python.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -32,6 +33,19 @@ PyObject* routing_address = nullptr;    // (routing or None, mask, M, stream) ->
 PyObject* ffn_bwd_workspace = nullptr;  // (a, d, h, row stride of the upstream gradient) -> workspace tensor
 PyObject* check = nullptr;              // (return code, function name): raises
 int64_t routed_min_rows = 0;            // below: no partition is shared
+
+// The MXFP4 operators' functions, ops' tensor class for them and the names of its slots (bind_mxfp4).
+struct MxLibrary {
+  decltype(&ffnk_mxfp4_quantise) quantise;
+  decltype(&ffnk_mxfp4_dequantise) dequantise;
+  decltype(&ffnk_mxfp4_workspace_bytes) workspace_bytes;
+  decltype(&ffnk_mxfp4_linear_fwd) linear_fwd;
+  decltype(&ffnk_mxfp4_linear_bwd) linear_bwd;
+  decltype(&ffnk_mxfp4_ffn_fwd) ffn_fwd;
+  decltype(&ffnk_mxfp4_ffn_bwd) ffn_bwd;
+} mx;
+PyTypeObject* mx_type = nullptr;
+PyObject *mx_codes, *mx_scales, *mx_columns, *mx_struct;  // slot names
 
 // _lib.PartitionStruct: memory for a row partition, and whether a launch that fills it has been made.
 struct Partition {
@@ -132,6 +146,9 @@ struct Call {
     r->made = 1;
     return true;
   }
+
+  // An MXFP4 tensor, of these extents where they are given (>= 0).
+  bool mxfp4(PyObject* o, int64_t r, int64_t c, struct Mxfp4* out);
 
  private:
   const at::Tensor* fail() {
@@ -271,22 +288,249 @@ PyObject* ffn_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+struct Mxfp4 {
+  int64_t rows = 0, columns = 0;
+  ffnk_mxfp4_t t{};
+};
+bool Call::mxfp4(PyObject* o, int64_t r, int64_t c, Mxfp4* out) {
+  if (!ok || !mx_type || Py_TYPE(o) != mx_type) return fail(), false;
+  THPObjectPtr codes(PyObject_GetAttr(o, mx_codes)), scales(PyObject_GetAttr(o, mx_scales)), columns(PyObject_GetAttr(o, mx_columns));
+  if (!codes || !scales || !columns) {
+    PyErr_Clear();
+    return fail(), false;
+  }
+  const at::Tensor *tc = strided(codes.get(), at::kByte, 2), *ts = strided(scales.get(), at::kByte, 2);
+  if (!tc || !ts) return false;
+  out->rows = tc->size(0);
+  out->columns = PyLong_AsLongLong(columns.get());
+  if (out->rows <= 0 || out->columns <= 0 || (r >= 0 && out->rows != r) || (c >= 0 && out->columns != c)) return fail(), false;
+  out->t = {static_cast<const uint8_t*>(tc->const_data_ptr()), static_cast<const uint8_t*>(ts->const_data_ptr())};
+  return true;
+}
+
+int dtype_id(at::ScalarType t) { return t == at::kBFloat16 ? FFNK_DT_BF16 : t == at::kHalf ? FFNK_DT_FP16 : t == at::kFloat ? FFNK_DT_FP32 : -1; }
+
+// (t) -> MXFP4
+PyObject* mx_quantise(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 1 || !mx_type || !THPVariable_CheckExact(p[0])) Py_RETURN_NOTIMPLEMENTED;
+  Call c;
+  const at::ScalarType type = THPVariable_Unpack(p[0]).scalar_type();
+  const at::Tensor* t = dtype_id(type) < 0 ? nullptr : c.strided(p[0], type, 2);
+  if (!t || !c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t rows = t->size(0), columns = t->size(1), nb = (columns + 31) / 32;
+  if (rows <= 0 || columns <= 1 || t->stride(1) != 1 || (rows > 1 && t->stride(0) < columns)) Py_RETURN_NOTIMPLEMENTED;
+  const auto bytes = t->options().dtype(at::kByte);
+  at::Tensor codes = at::empty({rows, nb * 16}, bytes), scales = at::empty({rows, (nb + 15) / 16 * 16}, bytes);
+  if (!run("ffnk_mxfp4_quantise", [&] {
+        const ffnk_mxfp4_t q{static_cast<const uint8_t*>(codes.mutable_data_ptr()), static_cast<const uint8_t*>(scales.mutable_data_ptr())};
+        return mx.quantise(t->const_data_ptr(), dtype_id(type), Call::ld(*t), &q, rows, columns, c.stream);
+      }))
+    return nullptr;
+  THPObjectPtr q(mx_type->tp_alloc(mx_type, 0)), a(THPVariable_Wrap(std::move(codes))), b(THPVariable_Wrap(std::move(scales))), k(PyLong_FromLongLong(columns));
+  if (!q || !a || !b || !k || PyObject_SetAttr(q.get(), mx_codes, a.get()) || PyObject_SetAttr(q.get(), mx_scales, b.get()) ||
+      PyObject_SetAttr(q.get(), mx_columns, k.get()) || PyObject_SetAttr(q.get(), mx_struct, Py_None))
+    return nullptr;
+  return q.release();
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, dtype) -> tensor
+PyObject* mx_dequantise(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2 || !THPDtype_Check(p[1])) Py_RETURN_NOTIMPLEMENTED;
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(p[1])->scalar_type;
+  Call c;
+  Mxfp4 q;
+  if (dtype_id(type) < 0 || !c.mxfp4(p[0], -1, -1, &q) || !c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor t = at::empty({q.rows, q.columns}, at::TensorOptions().device(at::Device(at::kCUDA, c.device)).dtype(type));
+  if (!run("ffnk_mxfp4_dequantise", [&] { return mx.dequantise(&q.t, t.mutable_data_ptr(), dtype_id(type), q.columns, q.rows, q.columns, c.stream); }))
+    return nullptr;
+  return THPVariable_Wrap(std::move(t));
+  END_HANDLE_TH_ERRORS
+}
+
+// The token rows of a forward: bf16 rows, or MXFP4 ones.
+struct MxInput {
+  const at::Tensor* x = nullptr;
+  Mxfp4 q;
+  int64_t columns = 0;
+  MxInput(Call* c, PyObject* o) {
+    if (mx_type && Py_TYPE(o) == mx_type) {
+      if (c->mxfp4(o, -1, -1, &q)) c->M = q.rows, columns = q.columns;
+    } else {
+      columns = size_of(o, 1);
+      x = c->rows(o, columns);
+    }
+  }
+  const uint16_t* rows() const { return x ? in(*x) : nullptr; }
+  int64_t stride() const { return x ? Call::ld(*x) : 0; }
+  const ffnk_mxfp4_t* held() const { return x ? nullptr : &q.t; }
+};
+at::Tensor mx_empty(const Call& c, int64_t r, int64_t k, at::ScalarType type = at::kBFloat16) {
+  return at::empty({r, k}, at::TensorOptions().device(at::Device(at::kCUDA, c.device)).dtype(type));
+}
+at::Tensor mx_workspace(const Call& c, size_t bytes) { return mx_empty(c, 1, (int64_t)(bytes > 16 ? bytes : 16), at::kByte); }
+
+// (a, b1, b2, mask, routing) -> c
+PyObject* mx_linear_fwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) Py_RETURN_NOTIMPLEMENTED;
+  Call c;
+  const MxInput a(&c, p[0]);
+  Mxfp4 b1, b2;
+  if (!c.mxfp4(p[1], -1, a.columns, &b1) || !c.mxfp4(p[2], b1.rows, a.columns, &b2)) Py_RETURN_NOTIMPLEMENTED;
+  const at::Tensor* mask = c.mask(p[3]);
+  if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t K = a.columns, N = b1.rows;
+  const size_t bytes = mx.workspace_bytes(FFNK_OP_LINEAR_FWD, c.M, K, N);
+  if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor y = mx_empty(c, c.M, N);
+  Partition* r;
+  if (!c.routing(p[4], p[3], &r)) return nullptr;
+  at::Tensor ws = mx_workspace(c, bytes);
+  if (!run("ffnk_mxfp4_linear_fwd", [&] {
+        return mx.linear_fwd(a.rows(), a.stride(), a.held(), &b1.t, &b2.t, static_cast<const uint8_t*>(mask->const_data_ptr()), out(y), N, c.M, K, N,
+                             ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r), r ? r->made : 1);
+      }))
+    return nullptr;
+  if (r) r->made = 1;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad, b1, b2, mask, routing) -> da
+PyObject* mx_linear_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) Py_RETURN_NOTIMPLEMENTED;
+  Call c;
+  const int64_t N = size_of(p[0], 1);
+  const at::Tensor* g = c.rows(p[0], N);
+  Mxfp4 b1, b2;
+  if (!c.mxfp4(p[1], N, -1, &b1) || !c.mxfp4(p[2], N, b1.columns, &b2)) Py_RETURN_NOTIMPLEMENTED;
+  const at::Tensor* mask = c.mask(p[3]);
+  if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t K = b1.columns;
+  const size_t bytes = mx.workspace_bytes(FFNK_OP_LINEAR_BWD, c.M, K, N);
+  if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor da = mx_empty(c, c.M, K);
+  Partition* r;
+  if (!c.routing(p[4], p[3], &r)) return nullptr;
+  at::Tensor ws = mx_workspace(c, bytes);
+  if (!c.fill(r, *mask)) return nullptr;
+  if (!run("ffnk_mxfp4_linear_bwd", [&] {
+        return mx.linear_bwd(in(*g), Call::ld(*g), &b1.t, &b2.t, static_cast<const uint8_t*>(mask->const_data_ptr()), out(da), K, c.M, K, N,
+                             ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r));
+      }))
+    return nullptr;
+  return THPVariable_Wrap(std::move(da));
+  END_HANDLE_TH_ERRORS
+}
+
+// Six weights of a feed-forward layer, w1 ... u3; d, h from the first.
+bool mx_ffn_weights(Call* c, PyObject* const* p, Mxfp4 (&w)[6], int64_t d) {
+  if (!c->mxfp4(p[0], -1, d, &w[0])) return false;
+  const int64_t h = w[0].rows;
+  for (int i = 1; i < 6; ++i)
+    if (!(i % 3 == 1 ? c->mxfp4(p[i], d, h, &w[i]) : c->mxfp4(p[i], h, d, &w[i]))) return false;
+  return true;
+}
+
+// (a, w1, w2, w3, u1, u2, u3, mask, save_pre, routing) -> out, or (out, pre) with save_pre
+PyObject* mx_ffn_fwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) Py_RETURN_NOTIMPLEMENTED;
+  Call c;
+  const MxInput a(&c, p[0]);
+  Mxfp4 w[6];
+  if (!c.ok || !mx_ffn_weights(&c, p + 1, w, a.columns)) Py_RETURN_NOTIMPLEMENTED;
+  const at::Tensor* mask = c.mask(p[7]);
+  if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t d = a.columns, h = w[0].rows;
+  const bool save = p[8] == Py_True;
+  const size_t bytes = mx.workspace_bytes(FFNK_OP_FFN_FWD, c.M, d, h);
+  if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor y = mx_empty(c, c.M, d), pre;
+  if (save) pre = mx_empty(c, c.M, 2 * h);
+  Partition* r;
+  if (!c.routing(p[9], p[7], &r)) return nullptr;
+  at::Tensor ws = mx_workspace(c, bytes);
+  if (!run("ffnk_mxfp4_ffn_fwd", [&] {
+        return mx.ffn_fwd(a.rows(), a.stride(), a.held(), &w[0].t, &w[1].t, &w[2].t, &w[3].t, &w[4].t, &w[5].t,
+                          static_cast<const uint8_t*>(mask->const_data_ptr()), out(y), d, save ? out(pre) : nullptr, c.M, d, h, ws.mutable_data_ptr(),
+                          (size_t)ws.numel(), c.stream, routing_of(r), r ? r->made : 1);
+      }))
+    return nullptr;
+  if (r) r->made = 1;
+  if (!save) return THPVariable_Wrap(std::move(y));
+  return Py_BuildValue("NN", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(pre)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad, w1, w2, w3, u1, u2, u3, mask, pre, routing) -> da
+PyObject* mx_ffn_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) Py_RETURN_NOTIMPLEMENTED;
+  Call c;
+  const int64_t d = size_of(p[0], 1);
+  const at::Tensor* g = c.rows(p[0], d);
+  Mxfp4 w[6];
+  if (!g || !mx_ffn_weights(&c, p + 1, w, d)) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t h = w[0].rows;
+  const at::Tensor *mask = c.mask(p[7]), *pre = c.rows(p[8], 2 * h);
+  if (pre && !pre->is_contiguous()) c.ok = false;
+  if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const size_t bytes = mx.workspace_bytes(FFNK_OP_FFN_BWD, c.M, d, h);
+  if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
+  at::Tensor da = mx_empty(c, c.M, d);
+  Partition* r;
+  if (!c.routing(p[9], p[7], &r)) return nullptr;
+  at::Tensor ws = mx_workspace(c, bytes);
+  if (!c.fill(r, *mask)) return nullptr;
+  if (!run("ffnk_mxfp4_ffn_bwd", [&] {
+        return mx.ffn_bwd(in(*g), Call::ld(*g), &w[0].t, &w[1].t, &w[2].t, &w[3].t, &w[4].t, &w[5].t, static_cast<const uint8_t*>(mask->const_data_ptr()),
+                          in(*pre), out(da), d, c.M, d, h, ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r));
+      }))
+    return nullptr;
+  return THPVariable_Wrap(std::move(da));
+  END_HANDLE_TH_ERRORS
+}
+
+bool addresses_into(PyObject* addresses, void* to, Py_ssize_t bytes) {
+  const Py_ssize_t n = bytes / (Py_ssize_t)sizeof(void*);
+  if (PyTuple_GET_SIZE(addresses) != n) {
+    PyErr_SetString(PyExc_ValueError, "bind: wrong number of functions");
+    return false;
+  }
+  void* f[16];
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, i));
+    if (!f[i]) return false;
+  }
+  memcpy(to, f, (size_t)bytes);
+  return true;
+}
+
+// (addresses of the library's functions in MxLibrary's order, the MXFP4 class); after bind
+PyObject* bind_mxfp4(PyObject*, PyObject* args) {
+  PyObject *addresses, *type;
+  if (!PyArg_ParseTuple(args, "O!O!", &PyTuple_Type, &addresses, &PyType_Type, &type)) return nullptr;
+  if (!addresses_into(addresses, &mx, sizeof(mx))) return nullptr;
+  PyObject** names[] = {&mx_codes, &mx_scales, &mx_columns, &mx_struct};
+  const char* const texts[] = {"_codes", "_scales", "_columns", "_struct"};
+  for (int i = 0; i < 4; ++i)
+    if (!*names[i] && !(*names[i] = PyUnicode_InternFromString(texts[i]))) return nullptr;
+  Py_INCREF(type);
+  Py_XSETREF(mx_type, reinterpret_cast<PyTypeObject*>(type));
+  Py_RETURN_NONE;
+}
+
 // (addresses of the library's functions in Library's order, routing_address, ffn_bwd_workspace, check, routed_min_rows)
 PyObject* bind(PyObject*, PyObject* args) {
   PyObject *addresses, *route, *space, *raise;
   long long rows;
   if (!PyArg_ParseTuple(args, "O!OOOL", &PyTuple_Type, &addresses, &route, &space, &raise, &rows)) return nullptr;
-  constexpr Py_ssize_t kFunctions = sizeof(Library) / sizeof(void*);
-  if (PyTuple_GET_SIZE(addresses) != kFunctions) {
-    PyErr_SetString(PyExc_ValueError, "bind: wrong number of functions");
-    return nullptr;
-  }
-  void* f[kFunctions];
-  for (Py_ssize_t i = 0; i < kFunctions; ++i) {
-    f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addresses, i));
-    if (!f[i]) return nullptr;
-  }
-  memcpy(&lib, f, sizeof(lib));
+  if (!addresses_into(addresses, &lib, sizeof(lib))) return nullptr;
   Py_INCREF(route);
   Py_INCREF(space);
   Py_INCREF(raise);
@@ -303,6 +547,13 @@ PyMethodDef methods[] = {
     {"linear_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(linear_bwd)), METH_FASTCALL, nullptr},
     {"ffn_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(ffn_fwd)), METH_FASTCALL, nullptr},
     {"ffn_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(ffn_bwd)), METH_FASTCALL, nullptr},
+    {"bind_mxfp4", bind_mxfp4, METH_VARARGS, nullptr},
+    {"mx_quantise", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_quantise)), METH_FASTCALL, nullptr},
+    {"mx_dequantise", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_dequantise)), METH_FASTCALL, nullptr},
+    {"mx_linear_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_linear_fwd)), METH_FASTCALL, nullptr},
+    {"mx_linear_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_linear_bwd)), METH_FASTCALL, nullptr},
+    {"mx_ffn_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_ffn_fwd)), METH_FASTCALL, nullptr},
+    {"mx_ffn_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mx_ffn_bwd)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods};
 

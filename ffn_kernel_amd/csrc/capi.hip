@@ -1469,6 +1469,13 @@ int api_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
 int api_check_extents(int64_t M, int64_t K, int64_t N) { return check_extents(M, K, N); }
 
 size_t routing_bytes(int64_t M) { return route_ws_bytes(M); }
+int routing_room(const ffnk_routing_t* caller, uint8_t* ws, int64_t M, const int32_t** perm, const int32_t** counts) {
+  if (caller != nullptr && (!caller->perm || !caller->counts)) return fail(FFNK_E_NULL, "routing: perm or counts is NULL");
+  const RouteWs r = carve_route(ws, M);
+  *perm = caller != nullptr ? caller->perm : r.perm;
+  *counts = caller != nullptr ? caller->counts : r.counts;
+  return FFNK_OK;
+}
 int make_routing(const ffnk_routing_t* caller, uint8_t* ws, const uint8_t* mask, int64_t M, hipStream_t stream, const int32_t** perm,
                  const int32_t** counts) {
   Routing rt;

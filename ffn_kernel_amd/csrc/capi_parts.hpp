@@ -21,6 +21,7 @@ int api_check_extents(int64_t M, int64_t K, int64_t N);
 
 // The partition a call works with: the caller's, or one made in `ws`, which holds routing_bytes(M).
 size_t routing_bytes(int64_t M);
+int routing_room(const ffnk_routing_t* caller, uint8_t* ws, int64_t M, const int32_t** perm, const int32_t** counts);  // made or not
 int make_routing(const ffnk_routing_t* caller, uint8_t* ws, const uint8_t* mask, int64_t M, hipStream_t stream, const int32_t** perm,
                  const int32_t** counts);
 

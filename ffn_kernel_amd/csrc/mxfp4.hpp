@@ -113,6 +113,9 @@ struct MxQuantiseArgs {
   const int32_t* perm;             // row r of the result is row perm[r] of x (NULL: row r)
   uint8_t *codes, *scales;
   int rows, columns;
+  // With a mask (rows entries) the launch also makes their partition, in blocks ahead of the others.
+  const uint8_t* mask = nullptr;
+  int32_t *part_perm = nullptr, *part_counts = nullptr;
 };
 hipError_t launch_mx_quantise(const MxQuantiseArgs& a, hipStream_t stream);
 struct MxDequantiseArgs {

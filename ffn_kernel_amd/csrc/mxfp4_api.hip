@@ -66,17 +66,53 @@ int check_ws(const void* ws, size_t have, size_t need) {
   return aligned(ws, 16) ? FFNK_OK : api_fail(FFNK_E_ALIGN, "workspace not 16-byte aligned");
 }
 
-// The call's rows as MXFP4: the caller's, or x quantised into `room` - in routed order where there is a partition, so that the GEMM
-// reads them row after row.
-int call_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const int32_t* perm, const Room& room, int64_t M, int64_t K,
-              hipStream_t stream, MxRows* out) {
+// The call's rows as MXFP4: the caller's, or x quantised into `room`.
+int stream_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const Room& room, int64_t M, int64_t K, hipStream_t stream, MxRows* out) {
   if (xq) {
     *out = rows_of(xq);
     return FFNK_OK;
   }
-  const MxQuantiseArgs q{x, x_stride_m, MX_BF16, perm, room.codes, room.scales, (int)M, (int)K};
+  const MxQuantiseArgs q{x, x_stride_m, MX_BF16, nullptr, room.codes, room.scales, (int)M, (int)K};
   FFNK_TRY_HIP(launch_mx_quantise(q, stream), "quantise kernel");
   *out = {room.codes, room.scales};
+  return FFNK_OK;
+}
+
+// ... with the partition (the caller's, or one in `ws`), which the quantising launch makes where it is still to be made.  The GEMM finds
+// its rows through it; where 32-bit offsets do not reach them, x is quantised in routed order instead.
+struct RoutedRows {
+  const int32_t *perm, *counts;
+  MxRows A;
+  int gather;
+};
+int routed_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const uint8_t* mask, const ffnk_routing_t* routing, int made, uint8_t* ws,
+                const Room& room, int64_t M, int64_t K, hipStream_t stream, RoutedRows* out) {
+  const bool reach = M * mx_code_stride(K) < k4g;
+  if (xq && !reach) return api_fail(FFNK_E_SHAPE, "xq: 32-bit offsets do not reach %lld rows of %lld columns", (long long)M, (long long)K);
+  if (int e = routing_room(routing, ws, M, &out->perm, &out->counts)) return e;
+  const bool make = routing == nullptr || !made;
+  int32_t *perm = const_cast<int32_t*>(out->perm), *counts = const_cast<int32_t*>(out->counts);
+  if (make && (xq || !reach)) FFNK_TRY_HIP(launch_route(mask, (int)M, perm, counts, stream), "route kernel");
+  out->gather = reach;
+  if (xq) {
+    out->A = rows_of(xq);
+    return FFNK_OK;
+  }
+  MxQuantiseArgs q{x, x_stride_m, MX_BF16, reach ? nullptr : perm, room.codes, room.scales, (int)M, (int)K};
+  if (make && reach) {
+    q.mask = mask;
+    q.part_perm = perm;
+    q.part_counts = counts;
+  }
+  FFNK_TRY_HIP(launch_mx_quantise(q, stream), "quantise kernel");
+  out->A = {room.codes, room.scales};
+  return FFNK_OK;
+}
+// Paths without a partition leave the caller's all the same.
+int leave_routing(const ffnk_routing_t* routing, int made, const uint8_t* mask, int64_t M, hipStream_t stream) {
+  if (routing == nullptr || made) return FFNK_OK;
+  if (!routing->perm || !routing->counts) return api_fail(FFNK_E_NULL, "routing: perm or counts is NULL");
+  FFNK_TRY_HIP(launch_route(mask, (int)M, const_cast<int32_t*>(routing->perm), const_cast<int32_t*>(routing->counts), stream), "route kernel");
   return FFNK_OK;
 }
 
@@ -203,10 +239,10 @@ size_t ffnk_mxfp4_workspace_bytes(int op, int64_t M, int64_t K, int64_t N) {
 
 int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const ffnk_mxfp4_t* Wv, const ffnk_mxfp4_t* Wt,
                           const uint8_t* mask, uint16_t* y, int64_t y_stride_m, int64_t M, int64_t K, int64_t N, void* ws, size_t ws_bytes,
-                          void* stream_, const ffnk_routing_t* routing) {
+                          void* stream_, const ffnk_routing_t* routing, int made) {
   hipStream_t stream = (hipStream_t)stream_;
   if (int e = check_call(M, K, N)) return e;
-  if (M == 0) return FFNK_OK;
+  if (M == 0) return leave_routing(routing, made, mask, M, stream);
   if (int e = check_rows(x, x_stride_m, xq, K)) return e;
   if (int e = check_tensor(Wv, "Wv")) return e;
   if (int e = check_tensor(Wt, "Wt")) return e;
@@ -216,30 +252,28 @@ int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp
   if (int e = check_ws(ws, ws_bytes, room.total)) return e;
   uint8_t* wsb = static_cast<uint8_t*>(ws);
   if (M <= kMxStreamRows) {
+    if (int e = leave_routing(routing, made, mask, M, stream)) return e;
     MxStreamArgs a{};
-    if (int e = call_rows(x, x_stride_m, xq, nullptr, carve_tensor(wsb, M, K), M, K, stream, &a.A)) return e;
+    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb, M, K), M, K, stream, &a.A)) return e;
     a.B0[0] = rows_of(Wv); a.B0[1] = rows_of(Wt);
     a.mask = mask; a.C = y; a.ldc = y_stride_m;
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
     FFNK_TRY_HIP(launch_mx_stream(a, stream), "MXFP4 stream");
     return FFNK_OK;
   }
-  if (xq && M * mx_code_stride(K) >= k4g) return api_fail(FFNK_E_SHAPE, "xq: 32-bit offsets do not reach %lld rows of %lld columns", (long long)M, (long long)K);
-  const int32_t *perm, *counts;
-  if (int e = make_routing(routing, wsb, mask, M, stream, &perm, &counts)) return e;
-  MxRows A;
-  if (int e = call_rows(x, x_stride_m, xq, perm, carve_tensor(wsb + room.x, M, K), M, K, stream, &A)) return e;
+  RoutedRows r;
+  if (int e = routed_rows(x, x_stride_m, xq, mask, routing, made, wsb, carve_tensor(wsb + room.x, M, K), M, K, stream, &r)) return e;
   const MxRows W[2] = {rows_of(Wv), rows_of(Wt)};
-  return tiled_product(room.plan, A, xq != nullptr, W, perm, counts, y, y_stride_m, M, K, N, reinterpret_cast<float*>(wsb + room.p), stream);
+  return tiled_product(room.plan, r.A, r.gather, W, r.perm, r.counts, y, y_stride_m, M, K, N, reinterpret_cast<float*>(wsb + room.p), stream);
 }
 
 int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2,
                        const ffnk_mxfp4_t* W3, const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
                        uint16_t* out, int64_t out_stride_m, uint16_t* pre, int64_t M, int64_t d, int64_t h, void* ws, size_t ws_bytes, void* stream_,
-                       const ffnk_routing_t* routing) {
+                       const ffnk_routing_t* routing, int made) {
   hipStream_t stream = (hipStream_t)stream_;
   if (int e = check_call(M, d, h)) return e;
-  if (M == 0) return FFNK_OK;
+  if (M == 0) return leave_routing(routing, made, mask, M, stream);
   if (int e = check_rows(x, x_stride_m, xq, d)) return e;
   const ffnk_mxfp4_t* weights[6] = {W1, W2, W3, U1, U2, U3};
   const char* names[6] = {"W1", "W2", "W3", "U1", "U2", "U3"};
@@ -253,8 +287,9 @@ int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t
   uint8_t* wsb = static_cast<uint8_t*>(ws);
   const Room hidden = carve_tensor(wsb + room.h, M, h);
   if (M <= kMxStreamRows && !pre) {
+    if (int e = leave_routing(routing, made, mask, M, stream)) return e;
     MxStreamArgs a{};
-    if (int e = call_rows(x, x_stride_m, xq, nullptr, carve_tensor(wsb + room.x, M, d), M, d, stream, &a.A)) return e;
+    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb + room.x, M, d), M, d, stream, &a.A)) return e;
     a.B0[0] = rows_of(W1); a.B0[1] = rows_of(U1); a.B1[0] = rows_of(W3); a.B1[1] = rows_of(U3);
     a.mask = mask; a.H = hidden.codes; a.SH = hidden.scales;
     a.M = (int)M; a.N = (int)h; a.K = (int)d;
@@ -267,21 +302,19 @@ int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t
     FFNK_TRY_HIP(launch_mx_stream(b, stream), "MXFP4 stream");
     return FFNK_OK;
   }
-  if (xq && M * mx_code_stride(d) >= k4g) return api_fail(FFNK_E_SHAPE, "xq: 32-bit offsets do not reach %lld rows of %lld columns", (long long)M, (long long)d);
-  const int32_t *perm, *counts;
-  if (int e = make_routing(routing, wsb, mask, M, stream, &perm, &counts)) return e;
+  RoutedRows r;
+  if (int e = routed_rows(x, x_stride_m, xq, mask, routing, made, wsb, carve_tensor(wsb + room.x, M, d), M, d, stream, &r)) return e;
   MxGemmArgs g{};
-  if (int e = call_rows(x, x_stride_m, xq, perm, carve_tensor(wsb + room.x, M, d), M, d, stream, &g.A)) return e;
-  g.gather = xq != nullptr;
+  g.A = r.A; g.gather = r.gather;
   g.B0[0] = rows_of(W1); g.B0[1] = rows_of(U1); g.B1[0] = rows_of(W3); g.B1[1] = rows_of(U3);
   g.H = hidden.codes; g.SH = hidden.scales;
   g.pre = pre; g.ld_pre = 2 * h;
-  g.perm = perm; g.counts = counts;
+  g.perm = r.perm; g.counts = r.counts;
   g.M = (int)M; g.N = (int)h; g.K = (int)d;
   g.splits = 1;
   FFNK_TRY_HIP(launch_mx_swiglu_gemm(room.up.tile, g, stream), "MXFP4 SwiGLU GEMM");
   const MxRows W[2] = {rows_of(W2), rows_of(U2)};
-  return tiled_product(room.down, {hidden.codes, hidden.scales}, false, W, perm, counts, out, out_stride_m, M, h, d,
+  return tiled_product(room.down, {hidden.codes, hidden.scales}, false, W, r.perm, r.counts, out, out_stride_m, M, h, d,
                        reinterpret_cast<float*>(wsb + room.p), stream);
 }
 

@@ -2,6 +2,7 @@
 #include <hip/hip_fp16.h>
 
 #include "mxfp4.hpp"
+#include "route_block.hpp"
 
 namespace ffnk {
 
@@ -29,6 +30,8 @@ struct MxElement<MX_FP32> {
   static __device__ __forceinline__ float load(T v) { return v; }
   static __device__ __forceinline__ T store(float v) { return v; }
 };
+
+static_assert(kRouteThreads == 256, "blocks of both kinds in one launch");
 
 template <class T>
 struct alignas(16) Run {
@@ -75,9 +78,16 @@ __device__ __forceinline__ float quad_lane(float v) {
 #endif
 }
 
-// U items of a lane, their loads in flight together.  VEC: rows are whole, aligned 16-byte pieces.
+// U items of a lane, their loads in flight together.  VEC: rows are whole, aligned 16-byte pieces.  The partition's blocks come first:
+// a launch of its own takes 3.3 us at M = 2048, and the GEMM behind both waits for either.
 template <int TYPE, int U, bool VEC>
-__global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a, const ItemShape shape, const int nb) {
+__global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a, const ItemShape shape, const int nb,
+                                                          const RouteShape route) {
+  if ((int)blockIdx.x < route.blocks) {
+    route_block(a.mask, a.rows, a.part_perm, a.part_counts, route.chunks_per_block, (int)blockIdx.x);
+    return;
+  }
+  const uint32_t block = blockIdx.x - (uint32_t)route.blocks;
   using E = MxElement<TYPE>;
   using T = typename E::T;
   constexpr int WG_ITEMS = 256 * U;
@@ -85,7 +95,7 @@ __global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a
   ItemAt at[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    at[u] = item_at<WG_ITEMS>(shape, blockIdx.x, u * 256 + (int)threadIdx.x);
+    at[u] = item_at<WG_ITEMS>(shape, block, u * 256 + (int)threadIdx.x);
     const int column = at[u].run * kItem;
 #pragma unroll
     for (int e = 0; e < kItem; ++e) v[u].v[e] = E::store(0.f);
@@ -183,13 +193,14 @@ hipError_t quantise(const MxQuantiseArgs& a, hipStream_t stream) {
   const int nb = (int)mx_blocks(a.columns), runs = 4 * nb;
   const bool vec = whole_runs(a.x, a.ldx, a.columns, TYPE), many = many_items(runs, a.rows);
   const ItemShape s = item_shape(runs, many ? 256 * kManyItems : 256);
-  const int64_t blocks = item_blocks(s, a.rows);
+  const RouteShape route = a.mask != nullptr ? route_shape(a.rows) : RouteShape{0, 0};
+  const int64_t blocks = item_blocks(s, a.rows) + route.blocks;
   if (blocks > 0xffffff) return hipErrorInvalidValue;  // (2^32 threads)
   const dim3 grid((unsigned)blocks), threads(256);
-  if (many && vec) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, kManyItems, true>), grid, threads, 0, stream, a, s, nb);
-  else if (many) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, kManyItems, false>), grid, threads, 0, stream, a, s, nb);
-  else if (vec) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, 1, true>), grid, threads, 0, stream, a, s, nb);
-  else hipLaunchKernelGGL((mx_quantise_kernel<TYPE, 1, false>), grid, threads, 0, stream, a, s, nb);
+  if (many && vec) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, kManyItems, true>), grid, threads, 0, stream, a, s, nb, route);
+  else if (many) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, kManyItems, false>), grid, threads, 0, stream, a, s, nb, route);
+  else if (vec) hipLaunchKernelGGL((mx_quantise_kernel<TYPE, 1, true>), grid, threads, 0, stream, a, s, nb, route);
+  else hipLaunchKernelGGL((mx_quantise_kernel<TYPE, 1, false>), grid, threads, 0, stream, a, s, nb, route);
   return hipGetLastError();
 }
 

@@ -19,8 +19,8 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from .ops import (Routing, _grad_mode, _on_device, _require_cuda_bf16, _require_mask, _route_cache, _routing_arg, _same_device,
+from . import _lib, ops
+from .ops import (Routing, _on_device, _require_cuda_bf16, _require_mask, _route_cache, _routing_arg, _same_device,
                   _stream_ptr, _workspace)
 
 _BLOCK = 32
@@ -39,7 +39,7 @@ class MXFP4:
     """A [rows, columns] tensor in MXFP4 on a GPU: `codes` uint8 [rows, 16 ceil(columns / 32)], two elements to a byte with the even
     column in the low half, and `scales` uint8 [rows, a multiple of 16], one exponent byte (bias 127) for 32 columns.  Bytes past the
     last column and the last block are 0: mxfp4_quantise and from_parts see to that, and the products count on it."""
-    __slots__ = ("_codes", "_scales", "_columns", "_struct", "_address")
+    __slots__ = ("_codes", "_scales", "_columns", "_struct")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
         for name, t, width in (("codes", codes, _code_bytes(columns)), ("scales", scales, _scale_bytes(columns))):
@@ -51,9 +51,7 @@ class MXFP4:
                 raise ValueError(f"{name} must be contiguous and 16-byte aligned")
         if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
             raise ValueError(f"codes are {tuple(codes.shape)} on {codes.device}, scales {tuple(scales.shape)} on {scales.device}")
-        self._codes, self._scales, self._columns = codes, scales, int(columns)
-        self._struct = _lib.Mxfp4Struct(codes.data_ptr(), scales.data_ptr())
-        self._address = ctypes.addressof(self._struct)
+        self._codes, self._scales, self._columns, self._struct = codes, scales, int(columns), None
 
     @classmethod
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int | None = None) -> "MXFP4":
@@ -77,6 +75,13 @@ class MXFP4:
     def __reduce__(self):
         return MXFP4, (self._codes, self._scales, self._columns)
 
+    @property
+    def _address(self) -> int:
+        """Of its ffnk_mxfp4_t."""
+        if self._struct is None:
+            self._struct = _lib.Mxfp4Struct(self._codes.data_ptr(), self._scales.data_ptr())
+        return ctypes.addressof(self._struct)
+
     codes = property(lambda self: self._codes)
     scales = property(lambda self: self._scales)
     columns = property(lambda self: self._columns)
@@ -89,6 +94,20 @@ class MXFP4:
 
     def __repr__(self):
         return f"MXFP4(shape={self.shape}, device='{self.device}')"
+
+
+_native_call = None
+
+
+def _native():
+    """_call.so with the MXFP4 functions bound (ops._native): they take the usual call and return NotImplemented for any other."""
+    global _native_call
+    if _native_call is None:
+        module, lib = ops._native(), _lib.load()
+        names = ("quantise", "dequantise", "workspace_bytes", "linear_fwd", "linear_bwd", "ffn_fwd", "ffn_bwd")
+        module.bind_mxfp4(tuple(ctypes.cast(getattr(lib, f"ffnk_mxfp4_{n}"), ctypes.c_void_p).value for n in names), MXFP4)
+        _native_call = module
+    return _native_call
 
 
 def _require_mxfp4(name: str, q) -> None:
@@ -110,6 +129,9 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
     """The rows of `t` ([rows, columns], bf16, fp16 or fp32) in MXFP4, in blocks of 32 columns (ffnk_mxfp4_quantise): the scale is the
     largest power of two not above the block's largest magnitude, over 4; elements go to the nearest number, ties to the even code,
     and saturate at 6.  A block with an infinity or a NaN is NaN.  The result carries no gradient."""
+    result = _native().mx_quantise(t)
+    if result is not NotImplemented:
+        return result
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"t must be a torch.Tensor, got {type(t).__name__}")
     if t.dim() != 2 or t.dtype not in _DTYPES:
@@ -129,6 +151,9 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
 
 def mxfp4_dequantise(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that `q` stands for, as a [rows, columns] tensor of bf16 (exact for normal numbers), fp16 or fp32."""
+    result = _native().mx_dequantise(q, dtype)
+    if result is not NotImplemented:
+        return result
     _require_mxfp4("q", q)
     if dtype not in _DTYPES:
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
@@ -174,6 +199,9 @@ def _check_differentiable(contraction: int, *extents: int) -> None:
 def masked_linear_mxfp4_forward(a, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
     """c[m] = Q(a[m]) @ (b1 if mask[m] else b2)^T.  a: bf16 [M, K] or MXFP4; b1, b2: MXFP4 [N, K]; routing: as in
     masked_linear_forward."""
+    result = _native().mx_linear_fwd(a, b1, b2, mask, routing)
+    if result is not NotImplemented:
+        return result
     a, x, ld, xq = _rows_of_call(a)
     M, K = a.shape
     dev = a.device
@@ -189,13 +217,16 @@ def masked_linear_mxfp4_forward(a, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, rou
         routing, rt = _routing_arg(routing, mask, M, stream)
         ws = _mx_workspace(_lib.OP_LINEAR_FWD, M, K, N, dev)
         rc = _lib.load().ffnk_mxfp4_linear_fwd(x, ld, xq, b1._address, b2._address, mask.data_ptr(), c.data_ptr(), N, M, K, N, ws.data_ptr(),
-                                               ws.numel(), stream, rt)
+                                               ws.numel(), stream, rt, 1)
     _lib.check(rc, "ffnk_mxfp4_linear_fwd")
     return c
 
 
 def masked_linear_mxfp4_backward(grad: torch.Tensor, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
     """da[m] = grad[m] @ (b1 if mask[m] else b2): the gradient of the rows over constant weights."""
+    result = _native().mx_linear_bwd(grad, b1, b2, mask, routing)
+    if result is not NotImplemented:
+        return result
     _require_cuda_bf16("grad", grad, 2)
     _require_mxfp4("b1", b1)
     M, dev = grad.shape[0], grad.device
@@ -240,6 +271,9 @@ def masked_ffn_mxfp4_forward(a, w1: MXFP4, w2: MXFP4, w3: MXFP4, u1: MXFP4, u2: 
     w1, w3, u1, u3: MXFP4 [h, d]; w2, u2: MXFP4 [d, h].
 
     save_pre: also return both projections, bf16 [M, 2h] in routed order (gate | up), for masked_ffn_mxfp4_backward."""
+    result = _native().mx_ffn_fwd(a, w1, w2, w3, u1, u2, u3, mask, bool(save_pre), routing)
+    if result is not NotImplemented:
+        return result
     a, x, ld, xq = _rows_of_call(a)
     M, dev = a.shape[0], a.device
     d, h = _check_ffn(a.shape, dev, w1, w2, w3, u1, u2, u3)
@@ -253,7 +287,8 @@ def masked_ffn_mxfp4_forward(a, w1: MXFP4, w2: MXFP4, w3: MXFP4, u1: MXFP4, u2: 
         routing, rt = _routing_arg(routing, mask, M, stream)
         ws = _mx_workspace(_lib.OP_FFN_FWD, M, d, h, dev)
         rc = _lib.load().ffnk_mxfp4_ffn_fwd(x, ld, xq, w1._address, w2._address, w3._address, u1._address, u2._address, u3._address, mask.data_ptr(),
-                                            out.data_ptr(), d, pre.data_ptr() if save_pre else None, M, d, h, ws.data_ptr(), ws.numel(), stream, rt)
+                                            out.data_ptr(), d, pre.data_ptr() if save_pre else None, M, d, h, ws.data_ptr(), ws.numel(), stream, rt,
+                                            1)
     _lib.check(rc, "ffnk_mxfp4_ffn_fwd")
     return (out, pre) if save_pre else out
 
@@ -262,6 +297,9 @@ def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP
                               pre: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
     """Gradient of the rows over constant weights: dh = grad @ w2, da = (dh * up * silu'(gate)) @ w1 + (dh * silu(gate)) @ w3, with the
     projections that masked_ffn_mxfp4_forward(..., save_pre=True) returned for the same mask."""
+    result = _native().mx_ffn_bwd(grad, w1, w2, w3, u1, u2, u3, mask, pre, routing)
+    if result is not NotImplemented:
+        return result
     _require_cuda_bf16("grad", grad, 2)
     M, dev = grad.shape[0], grad.device
     d, h = _check_ffn(grad.shape, dev, w1, w2, w3, u1, u2, u3)
@@ -285,33 +323,27 @@ def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP
     return da
 
 
-class _FrozenWeights(Function):
-    """Notes whether a gradient can be asked for: forward() itself always runs with gradients off."""
+def _gradient_wanted(a) -> bool:
+    return torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad
+
+
+class MaskedLinearMXFP4(Function):
+    """c = Q(a) @ (b1 where mask else b2)^T over MXFP4 weights [N, K]; differentiable in a bf16 `a`."""
 
     @classmethod
-    def apply(cls, *args):
-        _grad_mode.enabled = torch.is_grad_enabled()
-        return super().apply(*args)
-
-    @staticmethod
-    def _wanted(ctx) -> bool:
-        return _grad_mode.enabled and ctx.needs_input_grad[0]
-
-
-class MaskedLinearMXFP4(_FrozenWeights):
-    """c = Q(a) @ (b1 where mask else b2)^T over MXFP4 weights [N, K]; differentiable in a bf16 `a`."""
+    def apply(cls, a, b1, b2, mask):
+        # nothing to record: a third of a short call's host time is Function.apply's
+        return super().apply(a, b1, b2, mask) if _gradient_wanted(a) else masked_linear_mxfp4_forward(a, b1, b2, mask)
 
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
-        wanted = _FrozenWeights._wanted(ctx)
-        if wanted and isinstance(b1, MXFP4):
+        if isinstance(b1, MXFP4):
             _check_differentiable(*b1.shape)
         _route_cache.last = None
         out = masked_linear_mxfp4_forward(a, b1, b2, mask)
-        if wanted:
-            ctx.save_for_backward(mask)
-            ctx.weights = (b1, b2)
-            ctx.routing = _route_cache.last
+        ctx.save_for_backward(mask)
+        ctx.weights = (b1, b2)
+        ctx.routing = _route_cache.last
         return out
 
     @staticmethod
@@ -321,19 +353,22 @@ class MaskedLinearMXFP4(_FrozenWeights):
         return masked_linear_mxfp4_backward(grad, *ctx.weights, mask, routing=ctx.routing), None, None, None
 
 
-class MaskedFFNMXFP4(_FrozenWeights):
+class MaskedFFNMXFP4(Function):
     """Routed SwiGLU FFN over MXFP4 weights (w1, w3, u1, u3: [h, d]; w2, u2: [d, h]); differentiable in a bf16 `a`, for which the
     forward keeps both projections in bf16."""
+
+    @classmethod
+    def apply(cls, a, w1, w2, w3, u1, u2, u3, mask):
+        if _gradient_wanted(a):
+            return super().apply(a, w1, w2, w3, u1, u2, u3, mask)
+        return masked_ffn_mxfp4_forward(a, w1, w2, w3, u1, u2, u3, mask)
 
     @staticmethod
     def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
         weights = (w1, w2, w3, u1, u2, u3)
-        wanted = _FrozenWeights._wanted(ctx)
-        if wanted and isinstance(w2, MXFP4):
+        if isinstance(w2, MXFP4):
             _check_differentiable(*w2.shape)
         _route_cache.last = None
-        if not wanted:
-            return masked_ffn_mxfp4_forward(a, *weights, mask)
         out, pre = masked_ffn_mxfp4_forward(a, *weights, mask, save_pre=True)
         ctx.save_for_backward(mask, pre)
         ctx.weights = weights

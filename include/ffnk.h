@@ -464,11 +464,13 @@ FFNK_API int ffnk_mxfp4_dequantise(const ffnk_mxfp4_t* x, void* y, int dtype, in
 FFNK_API size_t ffnk_mxfp4_workspace_bytes(int op, int64_t M, int64_t K, int64_t N);
 
 /* y[m] = Q(x[m]) (mask[m] ? Wv : Wt)^T with the weights [N, K], as nn.Linear holds them.  The rows are bf16 x, quantised in the
- * call, or MXFP4 xq (the other is NULL).  fp32 sums, bf16 result.  routing as in ffnk_masked_linear_fwd_routed (M > 64). */
+ * call, or MXFP4 xq (the other is NULL).  fp32 sums, bf16 result.
+ * routing: the partition of `mask` to work with (NULL: one in the workspace); made == 0: it is still to be made, and the call
+ * leaves it there for the calls behind this one.  Up to 64 rows run without one. */
 FFNK_API int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq,
                                    const ffnk_mxfp4_t* Wv, const ffnk_mxfp4_t* Wt, const uint8_t* mask,
                                    uint16_t* y, int64_t y_stride_m, int64_t M, int64_t K, int64_t N,
-                                   void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+                                   void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing, int made);
 
 /* out[m] = Q(silu(Q(x[m]) W1^T) * (Q(x[m]) W3^T)) W2^T for visual rows, U1, U2, U3 for text rows; W1, W3 [h, d], W2 [d, h].
  * The intermediate goes from fp32 straight to MXFP4.  pre (optional, bf16 [M, 2h], 16-byte aligned where a backward reads it):
@@ -477,7 +479,7 @@ FFNK_API int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffn
                                 const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
                                 const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
                                 uint16_t* out, int64_t out_stride_m, uint16_t* pre, int64_t M, int64_t d, int64_t h,
-                                void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
+                                void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing, int made);
 
 /* Gradient of the rows over constant weights, the quantisations passed over (straight-through): dx[m] = g[m] W_grp.
  * K, N multiples of 8, N a multiple of 64 or at least 128; 16-byte aligned rows of g. */

@@ -129,16 +129,16 @@ def test_workspace_and_refusals_of_the_c_abi():
     assert quantise(None, 0, 0, None, 0, 32, None) == 0
     assert dequantise(q, None, 0, 32, 1, 32, None) == E["NULL"] and dequantise(q, 0x100, 0, 8, 1, 32, None) == E["STRIDE"]
     ws = (0x4000, 1 << 30)
-    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, None, 0, None, None) == E["WORKSPACE"]
-    assert linear(0x100, 64, q, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]      # x and xq
-    assert linear(None, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
-    assert linear(0x100, 64, None, q, None, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
-    assert linear(0x100, 64, None, q, q, None, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
-    assert linear(0x100, 63, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None) == E["STRIDE"]
-    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 63, 4, 64, 64, *ws, None, None) == E["STRIDE"]
-    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 0, 64, *ws, None, None) == E["SHAPE"]
-    assert linear(None, 0, q, q, q, 0x10, 0x100, 64, 1 << 24, 1 << 10, 64, 0x4000, 1 << 62, None, None) == E["SHAPE"]  # past 32-bit offsets
-    assert ffn(0x100, 64, None, q, q, q, q, q, None, 0x10, 0x100, 64, None, 4, 64, 64, *ws, None, None) == E["NULL"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, None, 0, None, None, 0) == E["WORKSPACE"]
+    assert linear(0x100, 64, q, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]      # x and xq
+    assert linear(None, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
+    assert linear(0x100, 64, None, q, None, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
+    assert linear(0x100, 64, None, q, q, None, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
+    assert linear(0x100, 63, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["STRIDE"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 63, 4, 64, 64, *ws, None, None, 0) == E["STRIDE"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 0, 64, *ws, None, None, 0) == E["SHAPE"]
+    assert linear(None, 0, q, q, q, 0x10, 0x100, 64, 1 << 24, 1 << 10, 64, 0x4000, 1 << 62, None, None, 0) == E["SHAPE"]  # past 32-bit offsets
+    assert ffn(0x100, 64, None, q, q, q, q, q, None, 0x10, 0x100, 64, None, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
     assert b"U3" in lib.ffnk_last_error()
     lb, fb = lib.ffnk_mxfp4_linear_bwd, lib.ffnk_mxfp4_ffn_bwd
     assert lb(0x100, 64, q, q, 0x10, 0x100, 63, 4, 63, 64, *ws, None, None) == E["STRIDE"]
@@ -146,4 +146,4 @@ def test_workspace_and_refusals_of_the_c_abi():
     assert lb(0x100, 64, q, q, 0x10, 0x100, 64, 4, 64, 64, 0x4000, 64, None, None) == E["WORKSPACE"]
     assert fb(0x100, 64, q, q, q, q, q, q, 0x10, None, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
     assert fb(0x100, 64, q, q, q, q, q, q, 0x10, 0x108, 0x100, 64, 4, 64, 64, *ws, None, None) == E["STRIDE"]
-    assert linear(None, 0, None, None, None, None, None, 64, 0, 64, 64, None, 0, None, None) == 0  # no rows
+    assert linear(None, 0, None, None, None, None, None, 64, 0, 64, 64, None, 0, None, None, 0) == 0  # no rows
