@@ -149,12 +149,14 @@ hipError_t launch_mx_swiglu_gemm(int tile, const MxGemmArgs& g, hipStream_t stre
 constexpr int kMxStreamRows = 64;
 struct MxStreamArgs {
   MxRows A;                        // [M, K], token order
+  const uint16_t* x; int64_t ldx;  // or bf16 rows, quantised by every workgroup (mx_stream_takes); NULL: A
   MxRows B0[2], B1[2];
   const uint8_t* mask;
   uint16_t* C; int64_t ldc;        // single weight: bf16 [M, N]
   uint8_t *H, *SH;                 // SwiGLU: MXFP4 [M, N], token order
   int M, N, K;
 };
+bool mx_stream_takes(int64_t M, int64_t K, const uint16_t* x, int64_t ldx);
 hipError_t launch_mx_stream(const MxStreamArgs& a, hipStream_t stream);
 hipError_t launch_mx_stream_swiglu(const MxStreamArgs& a, hipStream_t stream);
 

@@ -66,15 +66,20 @@ int check_ws(const void* ws, size_t have, size_t need) {
   return aligned(ws, 16) ? FFNK_OK : api_fail(FFNK_E_ALIGN, "workspace not 16-byte aligned");
 }
 
-// The call's rows as MXFP4: the caller's, or x quantised into `room`.
-int stream_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const Room& room, int64_t M, int64_t K, hipStream_t stream, MxRows* out) {
+// The rows of a streamed call: the caller's MXFP4 ones, bf16 ones that the stream quantises itself, or x quantised into `room`.
+int stream_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const Room& room, int64_t M, int64_t K, hipStream_t stream, MxStreamArgs* a) {
   if (xq) {
-    *out = rows_of(xq);
+    a->A = rows_of(xq);
+    return FFNK_OK;
+  }
+  if (mx_stream_takes(M, K, x, x_stride_m)) {
+    a->x = x;
+    a->ldx = x_stride_m;
     return FFNK_OK;
   }
   const MxQuantiseArgs q{x, x_stride_m, MX_BF16, nullptr, room.codes, room.scales, (int)M, (int)K};
   FFNK_TRY_HIP(launch_mx_quantise(q, stream), "quantise kernel");
-  *out = {room.codes, room.scales};
+  a->A = {room.codes, room.scales};
   return FFNK_OK;
 }
 
@@ -254,7 +259,7 @@ int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp
   if (M <= kMxStreamRows) {
     if (int e = leave_routing(routing, made, mask, M, stream)) return e;
     MxStreamArgs a{};
-    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb, M, K), M, K, stream, &a.A)) return e;
+    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb, M, K), M, K, stream, &a)) return e;
     a.B0[0] = rows_of(Wv); a.B0[1] = rows_of(Wt);
     a.mask = mask; a.C = y; a.ldc = y_stride_m;
     a.M = (int)M; a.N = (int)N; a.K = (int)K;
@@ -289,7 +294,7 @@ int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t
   if (M <= kMxStreamRows && !pre) {
     if (int e = leave_routing(routing, made, mask, M, stream)) return e;
     MxStreamArgs a{};
-    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb + room.x, M, d), M, d, stream, &a.A)) return e;
+    if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb + room.x, M, d), M, d, stream, &a)) return e;
     a.B0[0] = rows_of(W1); a.B0[1] = rows_of(U1); a.B1[0] = rows_of(W3); a.B1[1] = rows_of(U3);
     a.mask = mask; a.H = hidden.codes; a.SH = hidden.scales;
     a.M = (int)M; a.N = (int)h; a.K = (int)d;
