@@ -299,7 +299,7 @@ bool Call::mxfp4(PyObject* o, int64_t r, int64_t c, Mxfp4* out) {
     PyErr_Clear();
     return fail(), false;
   }
-  const at::Tensor *tc = strided(codes.get(), at::kByte, 2), *ts = strided(scales.get(), at::kByte, 2);
+  const at::Tensor *tc = strided(codes.get(), at::kByte, 2), *ts = strided(scales.get(), at::kByte, 3);
   if (!tc || !ts) return false;
   out->rows = tc->size(0);
   out->columns = PyLong_AsLongLong(columns.get());
@@ -321,7 +321,7 @@ PyObject* mx_quantise(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const int64_t rows = t->size(0), columns = t->size(1), nb = (columns + 31) / 32;
   if (rows <= 0 || columns <= 1 || t->stride(1) != 1 || (rows > 1 && t->stride(0) < columns)) Py_RETURN_NOTIMPLEMENTED;
   const auto bytes = t->options().dtype(at::kByte);
-  at::Tensor codes = at::empty({rows, nb * 16}, bytes), scales = at::empty({rows, (nb + 15) / 16 * 16}, bytes);
+  at::Tensor codes = at::empty({rows, nb * 16}, bytes), scales = at::empty({(nb + 15) / 16, rows, 16}, bytes);
   if (!run("ffnk_mxfp4_quantise", [&] {
         const ffnk_mxfp4_t q{static_cast<const uint8_t*>(codes.mutable_data_ptr()), static_cast<const uint8_t*>(scales.mutable_data_ptr())};
         return mx.quantise(t->const_data_ptr(), dtype_id(type), Call::ld(*t), &q, rows, columns, c.stream);

@@ -1,9 +1,11 @@
 // MXFP4 (OCP Microscaling): 32 neighbours of a row share a power-of-two scale, each is a 4-bit number.
 //   value = number * 2^(scale byte - 127),  numbers 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign (E2M1);  scale byte 255: NaN
 // A tensor of [rows, columns] is held as whole blocks: nb = cdiv(columns, 32) blocks of a row, 16 bytes of codes each (the even
-// column in a byte's low half), and one scale byte each in rows of mx_scale_stride(columns) bytes.  Codes past the last column
-// are 0; so are the scale bytes past the last block, which lets the products run over whole groups of blocks: a code read there
-// is some finite number, and the two operands' scales of 2^-127 take its product below the smallest fp32.
+// column in a byte's low half, rows one after the other), and one scale byte each.  The scale bytes of 16 blocks (512 columns) lie
+// together, and those of all rows behind one another, [cdiv(nb, 16)][rows][16]: the products want them for many rows at a time, and
+// a load of 64 rows of a tile is 1 KB in one piece instead of 64 cache lines.  Codes past the last column are 0; so are the scale
+// bytes past the last block, which lets the products run over whole groups of blocks: a code read there is some finite number, and
+// the two operands' scales of 2^-127 take its product below the smallest fp32.
 #pragma once
 #include "common.hpp"
 
@@ -16,7 +18,8 @@ constexpr int kMxBlock = 32;
 
 __host__ __device__ constexpr int64_t mx_blocks(int64_t columns) { return cdiv64(columns, kMxBlock); }
 __host__ __device__ constexpr int64_t mx_code_stride(int64_t columns) { return mx_blocks(columns) * 16; }
-__host__ __device__ constexpr int64_t mx_scale_stride(int64_t columns) { return round_up64(mx_blocks(columns), 16); }
+__host__ __device__ constexpr int64_t mx_scale_bytes(int64_t rows, int64_t columns) { return rows * round_up64(mx_blocks(columns), 16); }
+__host__ __device__ constexpr int64_t mx_scale_at(int64_t row, int64_t block, int64_t rows) { return (block / 16 * rows + row) * 16 + block % 16; }
 
 // Scale byte of a block whose largest magnitude is `top`: the largest power of two not above it over 4, the largest power of two of
 // the numbers, so that the largest one lands in [4, 8) and saturates at 6.  Blocks with an infinity or a NaN are NaN as a whole.
@@ -139,7 +142,7 @@ struct MxGemmArgs {
   int M, N, K;
   int splits; float* P;            // single weight, splits > 1: fp32 sums of a K range at P[split][p][N]
 };
-enum MxTileId : int { MX_256x256 = 0, MX_128x128 = 1 };
+enum MxTileId : int { MX_256x256 = 0, MX_128x256 = 1, MX_128x128 = 2, MX_64x128 = 3 };
 int mx_tile_rows(int tile);
 int mx_tile_columns(int tile, bool dual);  // output columns
 hipError_t launch_mx_gemm(int tile, const MxGemmArgs& g, hipStream_t stream);

@@ -25,7 +25,7 @@ int check_tensor(const ffnk_mxfp4_t* t, const char* name) {
 MxRows rows_of(const ffnk_mxfp4_t* t) { return {t->codes, t->scales}; }
 
 size_t tensor_bytes(int64_t rows, int64_t columns) {
-  return ws_align((size_t)(rows * mx_code_stride(columns))) + ws_align((size_t)(rows * mx_scale_stride(columns)));
+  return ws_align((size_t)(rows * mx_code_stride(columns))) + ws_align((size_t)mx_scale_bytes(rows, columns));
 }
 struct Room {
   uint8_t *codes, *scales;

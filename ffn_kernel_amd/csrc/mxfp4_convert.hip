@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a
           if (column + e < a.columns) v[u].v[e] = p[e];
     }
   }
-  const int64_t ldc = (int64_t)nb * 16, lds = round_up64(nb, 16);
+  const int64_t ldc = (int64_t)nb * 16;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float f[kItem], top = 0.f;
@@ -127,10 +127,10 @@ __global__ __launch_bounds__(256) void mx_quantise_kernel(const MxQuantiseArgs a
     *reinterpret_cast<uint32_t*>(a.codes + at[u].row * ldc + at[u].run * 4) = lo | (hi << 16);
     if ((at[u].run & 3) == 0) {
       const int b = at[u].run >> 2;
-      uint8_t* s = a.scales + at[u].row * lds;
-      s[b] = (uint8_t)byte;
+      uint8_t* s = a.scales + mx_scale_at(at[u].row, b, a.rows);
+      *s = (uint8_t)byte;
       if (b == nb - 1)
-        for (int64_t z = nb; z < lds; ++z) s[z] = 0;
+        for (int z = 1; (b + z) % 16 != 0; ++z) s[z] = 0;
     }
   }
 }
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void mx_dequantise_kernel(const MxDequantiseAr
   constexpr int WG_ITEMS = 256 * U;
   if (a.counts != nullptr && a.counts[blockIdx.y] == 0) return;
   const MxRows x = a.x[blockIdx.y];
-  const int64_t ldc = (int64_t)nb * 16, lds = round_up64(nb, 16);
+  const int64_t ldc = (int64_t)nb * 16;
   uint32_t codes[U], byte[U];
   ItemAt at[U];
 #pragma unroll
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(256) void mx_dequantise_kernel(const MxDequantiseAr
     codes[u] = byte[u] = 0;
     if (at[u].row < a.rows && at[u].run * kItem < a.columns) {
       codes[u] = *reinterpret_cast<const uint32_t*>(x.codes + at[u].row * ldc + at[u].run * 4);
-      byte[u] = x.scales[at[u].row * lds + (at[u].run >> 2)];
+      byte[u] = x.scales[mx_scale_at(at[u].row, at[u].run >> 2, a.rows)];
     }
   }
 #pragma unroll

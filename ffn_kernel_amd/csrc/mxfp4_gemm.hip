@@ -25,7 +25,7 @@ struct MxTile {
   static constexpr int LDS_BYTES = 2 * STAGE_BYTES + 2 * SCALE_BYTES;
   using Acc = f32x16_t;
   static_assert(LDS_BYTES <= 160 * 1024 && BM % 64 == 0 && (DUAL ? BN / 2 : BN) % 64 == 0 && WTN_OUT % 32 == 0 && WTM % 32 == 0, "tile");
-  static_assert((BM / 8) % NWAVES == 0 && (BN / 16) % NWAVES == 0, "panel rows spread evenly over the waves, gate and up rows apart");
+  static_assert((BM / 8) % NWAVES == 0 && (BN / (DUAL ? 16 : 8)) % NWAVES == 0, "panel rows spread evenly over the waves, gate and up rows apart");
 };
 
 __device__ __forceinline__ const uint8_t* wave_uniform(const uint8_t* p) {
@@ -43,15 +43,15 @@ template <class Cfg>
 struct MxLoop {
   static constexpr int NW = Cfg::NWAVES, TM = Cfg::TM, TN = Cfg::TN, BM = Cfg::BM, BN = Cfg::BN;
   static constexpr int NJA = TileLanes<Cfg>::NJA, NJB = TileLanes<Cfg>::NJB, LOADS = NJA + NJB;
-  static constexpr int NG = (BM + BN) / 64, NS = NG / NW;  // scale loads: 64 rows each
-  static_assert(NG % NW == 0, "every wave issues as many loads, which it counts");
+  // Scale loads: 64 rows each.  Every wave issues as many, which it counts: the last group's again where they do not come out even.
+  static constexpr int NG = (BM + BN) / 64, NS = cdiv(NG, NW);
   // A stage is four steps of 64 columns, TM x TN matrix instructions each.  Behind them, spread over the step, the next step's
   // fragments are read (the last step's early, the next stage's first ones behind the data barrier).  Two barriers a stage:
   //   RELEASE: every wave has read the last of this stage - the loads of the stage after next go into its memory from here on
   //   DATA: the next stage has landed
   // which leaves the loads 1.2 to 1.5 stages to land.
-  static constexpr int NM = TM * TN, NF = TM + TN, LEV = NM >= 16 ? 2 : 1;
-  static constexpr int RELEASE = 3 * NM - (NM >= 16 ? 4 : 1), DATA = 3 * NM + (NM >= 16 ? 6 : 1), TURN = 4 * NM;
+  static constexpr int NM = TM * TN, NF = TM + TN, LEV = NM >= 16 ? 2 : 1, EARLY = NM >= 16 ? 4 : NM >= 8 ? 2 : 1, LATE = NM >= 16 ? 6 : NM >= 8 ? 3 : 1;
+  static constexpr int RELEASE = 3 * NM - EARLY, DATA = 3 * NM + LATE, TURN = 4 * NM;
   static constexpr int FIRST = (TURN - RELEASE) / LEV, BEFORE = (DATA - RELEASE) / LEV;  // loads behind RELEASE in a stage, and of these ahead of DATA
   static_assert(FIRST <= LOADS && LOADS + NS - FIRST <= RELEASE / LEV, "the loads of a stage go out between its two RELEASE barriers");
 
@@ -65,6 +65,7 @@ struct MxLoop {
   uint32_t off_a[NJA], off_b[NJB], last_back;
   const uint8_t* scale_base[NS];
   uint32_t off_s[NS];
+  int64_t scale_turn[NS];  // from one 512 columns to the next
 
   __device__ __forceinline__ void init(const MxGemmArgs& g, uint8_t* lds_) {
     tl.init();
@@ -83,7 +84,7 @@ struct MxLoop {
   __device__ __forceinline__ void address(const MxGemmArgs& g, const TileCoord& tc, int first_stage, int end_stage) {
     kt0 = first_stage;
     kt1 = end_stage;
-    const int64_t lda = (int64_t)nb * 16, lds_row = round_up64(nb, 16);
+    const int64_t lda = (int64_t)nb * 16;
     // Gathered rows are addressed from the start of A (the host checks that 32 bits reach them).
     const int64_t row0 = g.gather ? 0 : tc.row0;
     const int n_first = min(tc.n0, g.N - 1);
@@ -105,17 +106,18 @@ struct MxLoop {
     // Scale rows: group q of 64, the token rows' first.
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      const int q = s * NW + tl.wave_s;  // (uniform)
+      const int q = min(s * NW + tl.wave_s, NG - 1);  // (uniform)
       if (q < BM / 64) {
-        scale_base[s] = g.A.scales + row0 * lds_row;
-        off_s[s] = (uint32_t)a_row(q * 64 + tl.lane) * (uint32_t)lds_row;
+        scale_base[s] = g.A.scales + row0 * 16;
+        off_s[s] = (uint32_t)a_row(q * 64 + tl.lane) * 16u;
       } else {
         const int r = q * 64 - BM;
         const bool up = Cfg::DUAL && r >= BN / 2;
-        scale_base[s] = (up ? g.B1[tc.grp].scales : g.B0[tc.grp].scales) + n_first * lds_row;
-        off_s[s] = (uint32_t)b_row(r - (up ? BN / 2 : 0) + tl.lane) * (uint32_t)lds_row;
+        scale_base[s] = (up ? g.B1[tc.grp].scales : g.B0[tc.grp].scales) + n_first * 16;
+        off_s[s] = (uint32_t)b_row(r - (up ? BN / 2 : 0) + tl.lane) * 16u;
       }
       scale_base[s] = wave_uniform(scale_base[s]);
+      scale_turn[s] = (int64_t)(q < BM / 64 ? g.M : g.N) * 16;
     }
   }
 
@@ -136,10 +138,10 @@ struct MxLoop {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(code_base[0]), FFNK_LDS_PTR(stage + (j * NW + tl.wave_s) * 1024), 16, off_a[j] + back,
                                                  kt * kRowBytes, 0, 0);
     } else {
-      const int s = l - LOADS, q = s * NW + tl.wave_s;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(scale_base[s]),
+      const int s = l - LOADS, q = min(s * NW + tl.wave_s, NG - 1);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(scale_base[s] + (kt >> 1) * scale_turn[s]),
                                                FFNK_LDS_PTR(lds + 2 * Cfg::STAGE_BYTES + ((kt >> 1) & 1) * Cfg::SCALE_BYTES + q * 1024), 16, off_s[s],
-                                               (kt >> 1) * 16, 0, 0);
+                                               0, 0, 0);
     }
   }
   // The loads ahead of the first stage: it whole, and of the second what the stage before would have issued.
@@ -270,7 +272,7 @@ template <class Cfg, bool WHOLE>  // WHOLE: no column past the last one
 __device__ __forceinline__ void mx_swiglu_store(const MxGemmArgs& g, const TileCoord& tc, const TileLanes<Cfg>& tl,
                                                 const f32x16_t (&acc)[Cfg::TM][Cfg::TN]) {
   const int nb = cdiv(g.N, kMxBlock);
-  const int64_t ldh = (int64_t)nb * 16, ldsh = round_up64(nb, 16);
+  const int64_t ldh = (int64_t)nb * 16;
 #pragma unroll
   for (int i = 0; i < Cfg::TM; ++i) {
     const int p = tc.row0 + tl.wm * Cfg::WTM + i * 32 + (int)tl.lr;
@@ -293,9 +295,12 @@ __device__ __forceinline__ void mx_swiglu_store(const MxGemmArgs& g, const TileC
       const u32x2_t w = lane_swap32(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
       if (p < tc.row_end && (WHOLE || b < nb)) {
         *reinterpret_cast<uint2*>(g.H + p * ldh + b * 16 + 8 * tl.lh) = make_uint2((w[0] & 0xffffu) | (w[1] << 16), (w[0] >> 16) | (w[1] & 0xffff0000u));
-        if (tl.lh == 0) g.SH[p * ldsh + b] = (uint8_t)byte;
-        if (tl.lh == 0 && b == nb - 1)
-          for (int64_t z = nb; z < ldsh; ++z) g.SH[p * ldsh + z] = 0;
+        if (tl.lh == 0) {
+          uint8_t* s = g.SH + mx_scale_at(p, b, g.M);
+          *s = (uint8_t)byte;
+          if (b == nb - 1)
+            for (int z = 1; (b + z) % 16 != 0; ++z) s[z] = 0;
+        }
       }
     }
   }
@@ -393,23 +398,28 @@ hipError_t launch(const MxGemmArgs& g, hipStream_t stream) {
 
 template <bool DUAL>
 struct MxTiles {
-  using Big = MxTile<256, 256, 2, 2, DUAL, DUAL ? 8 : 4>;
-  using Small = MxTile<128, 128, 2, 2, DUAL, DUAL ? 8 : 4>;
+  static constexpr int G = DUAL ? 8 : 4;
+  using T0 = MxTile<256, 256, 2, 2, DUAL, G>;
+  using T1 = MxTile<128, 256, 2, 2, DUAL, G>;
+  using T2 = MxTile<128, 128, 2, 2, DUAL, G>;
+  using T3 = MxTile<64, 128, 2, 2, DUAL, G>;
 };
 
 template <bool DUAL>
 hipError_t dispatch(int tile, const MxGemmArgs& g, hipStream_t stream) {
   switch (tile) {
-    case MX_256x256: return launch<typename MxTiles<DUAL>::Big>(g, stream);
-    case MX_128x128: return launch<typename MxTiles<DUAL>::Small>(g, stream);
+    case MX_256x256: return launch<typename MxTiles<DUAL>::T0>(g, stream);
+    case MX_128x256: return launch<typename MxTiles<DUAL>::T1>(g, stream);
+    case MX_128x128: return launch<typename MxTiles<DUAL>::T2>(g, stream);
+    case MX_64x128: return launch<typename MxTiles<DUAL>::T3>(g, stream);
     default: return hipErrorInvalidValue;
   }
 }
 
 }  // namespace
 
-int mx_tile_rows(int tile) { return tile == MX_256x256 ? 256 : 128; }
-int mx_tile_columns(int tile, bool dual) { return (tile == MX_256x256 ? 256 : 128) / (dual ? 2 : 1); }
+int mx_tile_rows(int tile) { return tile == MX_256x256 ? 256 : tile == MX_64x128 ? 64 : 128; }
+int mx_tile_columns(int tile, bool dual) { return (tile == MX_256x256 || tile == MX_128x256 ? 256 : 128) / (dual ? 2 : 1); }
 
 hipError_t launch_mx_gemm(int tile, const MxGemmArgs& g, hipStream_t stream) { return dispatch<false>(tile, g, stream); }
 hipError_t launch_mx_swiglu_gemm(int tile, const MxGemmArgs& g, hipStream_t stream) { return dispatch<true>(tile, g, stream); }

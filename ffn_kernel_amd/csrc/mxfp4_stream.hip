@@ -74,7 +74,8 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
   for (int t = 0; t < NT; ++t) token[t] = __shfl(job.token, min(t * 16 + lr, rows - 1));  // rows past the last repeat it; not stored
 
   const int nb = cdiv(a.K, kMxBlock), groups = cdiv(a.K, kGroupK);
-  const int64_t ld = (int64_t)nb * 16, ld_s = round_up64(nb, 16);
+  const int64_t ld = (int64_t)nb * 16;
+  const int pad = cdiv(nb, 16) * 16 - nb;
   const int n0 = (int)blockIdx.x * TILES * 16;
 
   f32x4_t acc[NW][NT];
@@ -96,8 +97,8 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
     for (int r = 0; r < NW; ++r) {
       const MxRows& w = DUAL && r >= TILES ? a.B1[grp] : a.B0[grp];
       const int first = min(n0 + (r % TILES) * 16, a.N - 1), left = a.N - 1 - first;  // (uniform)
-      const uint8_t *codes = w.codes + first * ld, *scales = w.scales + first * ld_s + g * 16;
-      v.scales[r] = *reinterpret_cast<const i32x4_t*>(scales + (uint32_t)min(lr, left) * (uint32_t)ld_s);
+      const uint8_t *codes = w.codes + first * ld, *scales = w.scales + ((int64_t)g * a.N + first) * 16;
+      v.scales[r] = *reinterpret_cast<const i32x4_t*>(scales + min(lr, left) * 16);
 #pragma unroll
       for (int q = 0; q < 4; ++q) v.codes[r][q] = __builtin_nontemporal_load(reinterpret_cast<const i32x4_t*>(codes + ((uint32_t)min(4 * q + lg, left) * (uint32_t)ld + piece)));
     }
@@ -109,12 +110,12 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
       const uint8_t *codes, *scales;
       if constexpr (FUSED) {
         codes = job.fused + min(lr, rows - 1) * fused_code_stride(nb);
-        scales = job.fused + kFusedRows * fused_code_stride(nb) + min(lr, rows - 1) * fused_scale_stride(nb);
+        scales = job.fused + kFusedRows * fused_code_stride(nb) + min(lr, rows - 1) * fused_scale_stride(nb) + g * 16;
       } else {
         codes = a.A.codes + token[t] * ld;
-        scales = a.A.scales + token[t] * ld_s;
+        scales = a.A.scales + ((int64_t)g * a.M + token[t]) * 16;
       }
-      v.scales[t] = *reinterpret_cast<const i32x4_t*>(scales + g * 16);
+      v.scales[t] = *reinterpret_cast<const i32x4_t*>(scales);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v.codes[t][i] = *reinterpret_cast<const i32x4_t*>(codes + min(g * kGroupBlocks + 4 * i + lg, nb - 1) * 16);
     }
@@ -164,9 +165,9 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
     };
     auto put_rows = [&]() {
       // scale bytes behind the last block
-      for (int z = (int)threadIdx.x; z < rows * (int)(ld_s - nb); z += NTHREADS) {
-        const int r = z / (int)(ld_s - nb);
-        job.fused[kFusedRows * fused_code_stride(nb) + r * fused_scale_stride(nb) + nb + z - r * (int)(ld_s - nb)] = 0;
+      for (int z = (int)threadIdx.x; z < rows * pad; z += NTHREADS) {
+        const int r = z / pad;
+        job.fused[kFusedRows * fused_code_stride(nb) + r * fused_scale_stride(nb) + nb + z - r * pad] = 0;
       }
       put_block((int)threadIdx.x);
       for (int first = NTHREADS; first < blocks; first += NTHREADS) {
@@ -241,7 +242,7 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
   if constexpr (DUAL) {
     static_assert(TILES == 2, "a block of the intermediate");
     const int nbh = cdiv(a.N, kMxBlock), b = (int)blockIdx.x;
-    const int64_t ldh = (int64_t)nbh * 16, ldsh = round_up64(nbh, 16);
+    const int64_t ldh = (int64_t)nbh * 16;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (t * 16 >= rows) continue;
@@ -259,10 +260,10 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
       *reinterpret_cast<uint16_t*>(hc) = (uint16_t)mx_codes4(h[0], h[1], h[2], h[3], byte);
       *reinterpret_cast<uint16_t*>(hc + 8) = (uint16_t)mx_codes4(h[4], h[5], h[6], h[7], byte);
       if (lg == 0) {
-        uint8_t* hs = a.SH + token[t] * ldsh;
-        hs[b] = (uint8_t)byte;
+        uint8_t* s = a.SH + mx_scale_at(token[t], b, a.M);
+        *s = (uint8_t)byte;
         if (b == nbh - 1)
-          for (int64_t z = nbh; z < ldsh; ++z) hs[z] = 0;
+          for (int z = 1; (b + z) % 16 != 0; ++z) s[z] = 0;
       }
     }
   } else {

@@ -74,7 +74,7 @@ class _MXFP4Weights(nn.Module):
         for name, (rows, columns) in shapes.items():
             blocks = -(-columns // 32)
             self.register_buffer(f"{name}_codes", torch.zeros((rows, 16 * blocks), dtype=torch.uint8, device=device))
-            self.register_buffer(f"{name}_scales", torch.zeros((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=device))
+            self.register_buffer(f"{name}_scales", torch.zeros((-(-blocks // 16), rows, 16), dtype=torch.uint8, device=device))
 
     def _quantise(self, weights: dict) -> None:
         for name, w in weights.items():

@@ -31,26 +31,28 @@ def _code_bytes(columns: int) -> int:
     return -(-columns // _BLOCK) * 16
 
 
-def _scale_bytes(columns: int) -> int:
-    return -(-columns // (_BLOCK * 16)) * 16
+def _scale_shape(rows: int, columns: int) -> tuple:
+    return (-(-columns // (_BLOCK * 16)), rows, 16)
 
 
 class MXFP4:
     """A [rows, columns] tensor in MXFP4 on a GPU: `codes` uint8 [rows, 16 ceil(columns / 32)], two elements to a byte with the even
-    column in the low half, and `scales` uint8 [rows, a multiple of 16], one exponent byte (bias 127) for 32 columns.  Bytes past the
-    last column and the last block are 0: mxfp4_quantise and from_parts see to that, and the products count on it."""
+    column in the low half, and `scales` uint8 [ceil(columns / 512), rows, 16], one exponent byte (bias 127) for 32 columns: those of
+    512 columns together, and of all rows behind one another, as the products load them (parts() has them row by row).  Bytes past
+    the last column and the last block are 0: mxfp4_quantise and from_parts see to that, and the products count on it."""
     __slots__ = ("_codes", "_scales", "_columns", "_struct")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
-        for name, t, width in (("codes", codes, _code_bytes(columns)), ("scales", scales, _scale_bytes(columns))):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != width:
-                raise ValueError(f"{name} must be a torch.uint8 tensor [rows, {width}] for {columns} columns")
+        rows = codes.shape[0] if isinstance(codes, torch.Tensor) and codes.dim() == 2 else 0
+        for name, t, shape in (("codes", codes, (rows, _code_bytes(columns))), ("scales", scales, _scale_shape(rows, columns))):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.shape != shape:
+                raise ValueError(f"{name} must be a torch.uint8 tensor {list(shape)} for {rows} rows of {columns} columns")
             if not t.is_cuda:
                 raise ValueError(f"{name} must live on a GPU (got {t.device}); libffnk has no CPU path")
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"{name} must be contiguous and 16-byte aligned")
-        if codes.shape[0] != scales.shape[0] or codes.device != scales.device:
-            raise ValueError(f"codes are {tuple(codes.shape)} on {codes.device}, scales {tuple(scales.shape)} on {scales.device}")
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
         self._codes, self._scales, self._columns, self._struct = codes, scales, int(columns), None
 
     @classmethod
@@ -65,12 +67,17 @@ class MXFP4:
         if columns < 0 or codes.shape[1] < held or scales.shape[1] < blocks:
             raise ValueError(f"{columns} columns need {held} bytes of codes and {blocks} scales a row, got {codes.shape[1]} and {scales.shape[1]}")
         new_codes = torch.zeros((rows, _code_bytes(columns)), dtype=torch.uint8, device=codes.device)
-        new_scales = torch.zeros((rows, _scale_bytes(columns)), dtype=torch.uint8, device=codes.device)
+        new_scales = torch.zeros((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=codes.device)
         new_codes[:, :held] = codes[:, :held]
         if columns % 2:
             new_codes[:, held - 1] &= 15
         new_scales[:, :blocks] = scales[:, :blocks]
-        return cls(new_codes, new_scales, columns)
+        return cls(new_codes, new_scales.view(rows, -1, 16).transpose(0, 1).contiguous(), columns)
+
+    def parts(self) -> tuple:
+        """(codes [rows, 16 ceil(columns / 32)], scales [rows, ceil(columns / 32)]): what from_parts takes, the scales as a copy."""
+        rows, columns = self.shape
+        return self._codes, self._scales.transpose(0, 1).reshape(rows, -1)[:, :-(-columns // _BLOCK)]
 
     def __reduce__(self):
         return MXFP4, (self._codes, self._scales, self._columns)
@@ -142,7 +149,7 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
     rows, columns = t.shape
     with _on_device(t.device):
         codes = torch.empty((rows, _code_bytes(columns)), dtype=torch.uint8, device=t.device)
-        scales = torch.empty((rows, _scale_bytes(columns)), dtype=torch.uint8, device=t.device)
+        scales = torch.empty(_scale_shape(rows, columns), dtype=torch.uint8, device=t.device)
         q = MXFP4(codes, scales, columns)
         _lib.check(_lib.load().ffnk_mxfp4_quantise(t.data_ptr(), _DTYPES[t.dtype], _row_stride(t), q._address, rows, columns,
                                                    _stream_ptr(t.device)), "ffnk_mxfp4_quantise")

@@ -439,8 +439,10 @@ FFNK_API int ffnk_masked_ffn_bwd_routed(const uint16_t* g, int64_t g_stride_m,
  * A tensor of [rows, columns] holds its rows in blocks of 32 columns, nb = ceil(columns / 32) of them.  An element is
  * E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times the block's scale, 2^(byte - 127) (E8M0; byte 255: the block is NaN).
  *   codes:  rows of 16 * nb bytes, two elements to a byte, the even column in the low half; 0 behind the last column
- *   scales: rows of 16 * ceil(nb / 16) bytes, one for each block; 0 behind the last block (the products rely on it)
- * Rows follow one another without gaps; both pointers are 16-byte aligned device memory.
+ *           (rows follow one another without gaps)
+ *   scales: [ceil(nb / 16)][rows][16] bytes, one for each block: those of 512 columns together, and of all rows behind one another;
+ *           0 behind the last block (the products rely on it)
+ * Both pointers are 16-byte aligned device memory.
  */
 typedef struct ffnk_mxfp4_t {
   const uint8_t* codes;
