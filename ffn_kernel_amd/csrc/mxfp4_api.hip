@@ -32,22 +32,54 @@ struct Room {
 };
 Room carve_tensor(uint8_t* ws, int64_t rows, int64_t columns) { return {ws, ws + ws_align((size_t)(rows * mx_code_stride(columns)))}; }
 
-// Tile and K ranges of a GEMM over [M, K] x [N, K]^T.
+// Tile and K ranges of a GEMM over [M, K] x [N, K]^T: the cheapest by a model of the launch, in us.  A round of tiles (`slots` at once)
+// costs a fixed time and a time per stage of 256 columns, both at most half full and quite full, in between by its share.  The costs are
+// fits to (256x256 / 128x256 / 128x128 / 64x128, single weight, half of the rows in either modality)
+//   M 4096, N 4096, K 14336  110 / 130 / 129 / 197      M 8192, N = K = 2048  28.1 / 31.7 / 28.2 / 37.3
+//   M 1411, N 4096, K 14336  77.4 / 52.9 / 53.6 / 74.5  M 8192, N = K = 1024  18.5 / 14.3 / 12.5 / 14.7
+//   M 300, N 4096, K 14336   68.0 / 44.6 / 35.6 / 33.4  M 2048, N = K = 1024  16.2 / 10.5 / 7.6 / 6.9
+// and, with an eighth more for the smaller tiles, SwiGLU's (K = 4096, 14336 columns): M = 300 38.0 / 46.2 / 44.3 / 52.4, M = 700
+// 71.9 / 70.3 / 66.7 / 98.9, M = 1411 124.7 / 138.8 / 130.6 / 187.8.
+// K ranges add a pass over their sums: M = 300, N 4096, K 14336 in four ranges of 128x128 26.8 and 5.0.
 struct Plan {
   int tile, splits;
 };
-int64_t tiles_of(int tile, bool dual, int64_t M, int64_t N) { return (cdiv64(M, mx_tile_rows(tile)) + 1) * cdiv64(N, mx_tile_columns(tile, dual)); }
+struct TileCost {
+  int slots;
+  float fixed, stage, fixed_full, stage_full;
+};
+constexpr TileCost kTileCosts[] = {{256, 12.7f, 0.96f, 14.5f, 1.7f}, {256, 8.f, 0.63f, 11.f, 0.95f}, {512, 5.f, 0.5f, 7.5f, 1.05f}, {512, 4.5f, 0.5f, 4.f, 0.8f}};
+float launch_us(const TileCost& c, int64_t workgroups, float stages) {
+  const float half = c.fixed + stages * c.stage, full = c.fixed_full + stages * c.stage_full;
+  const float share = (float)(workgroups % c.slots) / (float)c.slots;
+  return (float)(workgroups / c.slots) * full + (share == 0.f ? 0.f : share <= 0.5f ? half : half + (full - half) * (2.f * share - 1.f));
+}
 Plan plan_gemm(bool dual, int64_t M, int64_t N, int64_t K) {
-  Plan p{MX_128x128, 1};
-  if (tiles_of(MX_256x256, dual, M, N) >= kCusPerChip) p.tile = MX_256x256;
-  else if (!dual && N % 4 == 0 && M < 65536) {
-    const int64_t tiles = tiles_of(MX_128x128, dual, M, N), chunks = cdiv64(K, 512);
-    int64_t s = 2 * kCusPerChip / tiles;
-    if (s > chunks / 4) s = chunks / 4;
-    if (s > kMaxSplits) s = kMaxSplits;
-    if (s > 1) p.splits = (int)cdiv64(chunks, cdiv64(chunks, s));  // no empty range
+  const int64_t pairs = cdiv64(K, 512);  // two stages each: K ranges are whole pairs
+  Plan best{MX_256x256, 1};
+  float best_us = 1e30f;
+  for (int tile = MX_256x256; tile <= MX_64x128; ++tile) {
+    const TileCost& c = kTileCosts[tile];
+    // The mask decides between cdiv(M, rows) M-tiles and one more, which it is where the first modality's rows leave fewer past their
+    // whole tiles than all rows do.
+    const int64_t rows = mx_tile_rows(tile), tiles_n = cdiv64(N, mx_tile_columns(tile, dual)), fewer = cdiv64(M, rows) * tiles_n, tiles = fewer + tiles_n;
+    const float more = (float)(M - (cdiv64(M, rows) - 1) * rows) / (float)rows;
+    if (tile != MX_256x256 && tiles > kMxMaxWorkgroups) break;
+    for (int splits = 1; splits <= kMaxSplits; ++splits) {
+      if (splits > 1 && (dual || N % 4 != 0 || M >= 65536 || splits * 2 > pairs || tiles * splits > c.slots)) break;
+      const int64_t per_range = cdiv64(pairs, splits);
+      if (per_range * (splits - 1) >= pairs) continue;  // an empty range
+      const float stages = splits > 1 ? (float)(2 * per_range) : (float)cdiv64(K, 256);
+      float us = (1.f - more) * launch_us(c, fewer * splits, stages) + more * launch_us(c, tiles * splits, stages);
+      if (dual && tile != MX_256x256) us *= 1.125f;
+      if (splits > 1) us += 2.5f + (float)(splits * M * N) * 4.f / 4e6f;
+      if (us < best_us) {
+        best_us = us;
+        best = {tile, splits};
+      }
+    }
   }
-  return p;
+  return best;
 }
 size_t partial_bytes(const Plan& p, int64_t M, int64_t N) { return p.splits > 1 ? ws_align((size_t)p.splits * M * N * 4) : 0; }
 

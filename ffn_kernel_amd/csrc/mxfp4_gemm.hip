@@ -384,7 +384,7 @@ hipError_t launch(const MxGemmArgs& g, hipStream_t stream) {
   const int pairs = cdiv(cdiv(g.K, kMxStageK), 2);
   if ((g.splits - 1) * cdiv(pairs, g.splits) >= pairs) return hipErrorInvalidValue;  // an empty K range
   const int64_t total = (int64_t)(cdiv(g.M, Cfg::BM) + 1) * cdiv(g.N, Cfg::BN_OUT) * g.splits;
-  if (total > 0xffff00) return hipErrorInvalidValue;  // (2^32 threads)
+  if (total > kMxMaxWorkgroups) return hipErrorInvalidValue;
   const dim3 blocks((unsigned)round_up64(total, kXcds));
   if constexpr (Cfg::DUAL) {
     if (g.pre != nullptr) {
