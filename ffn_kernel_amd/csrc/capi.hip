@@ -1504,14 +1504,13 @@ namespace {
 struct FfnDxPlan {
   int64_t half;
   RoutedPlan dx;
-  size_t dx_need, off_dh, off_p, total;
+  size_t dx_need, off_p, total;
 };
 FfnDxPlan plan_ffn_dx(int64_t M, int64_t d, int64_t h) {
   FfnDxPlan p;
   p.half = round_up64(h, 64);
   p.dx = ffn_bwd_dx_plan(M, d, 2 * p.half, true, 2 * ws_align((size_t)h * d * 2), &p.dx_need);
-  p.off_dh = ws_align((size_t)M * 2 * p.half * 2);
-  p.off_p = p.off_dh + ws_align((size_t)M * h * 2);
+  p.off_p = ws_align((size_t)M * 2 * p.half * 2);
   p.total = p.off_p + ws_align(p.dx_need);
   return p;
 }
@@ -1531,7 +1530,7 @@ int ffn_dx(const uint16_t* g, int64_t g_stride_m, const uint16_t* pre, const uin
   GemmArgs a;
   a.A = g; a.lda = g_stride_m;
   a.B0[0] = W2[0]; a.B0[1] = W2[1]; a.B1[0] = a.B1[1] = nullptr; a.ldb = h;
-  a.C = reinterpret_cast<uint16_t*>(ws + p.off_dh); a.ldc = h;
+  a.C = nullptr; a.ldc = h;  // (the intermediate: only weight gradients need it)
   a.perm = perm; a.counts = counts;
   a.M = (int)M; a.N = (int)h; a.K = (int)d; a.group_m = plan_group_m(TUNED_NONE, M, d, h);
   a.pre = pre; a.ld_pre = 2 * h; a.half_pre = (int)h;

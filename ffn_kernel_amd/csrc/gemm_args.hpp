@@ -30,7 +30,7 @@ struct GemmArgs {
   // Gather kernels only (GATHER_A, rows of C in routed order), SwiGLU backward instead of the plain result: always over K-major weights, by
   // choice over row-major ones.  With
   // dh = A B0^T, t1 = pre[row, n], t3 = pre[row, half_pre + n] (rows in routed order):
-  //   T13[row, n] = dh * t3 * silu'(t1),  T13[row, half + n] = dh * silu(t1),  C[row, n] = silu(t1) * t3   for n < N
+  //   T13[row, n] = dh * t3 * silu'(t1),  T13[row, half + n] = dh * silu(t1),  C[row, n] = silu(t1) * t3   for n < N (C NULL: not stored)
   //   T13[row, n] = T13[row, half + n] = 0                                                                 for N <= n < half
   // pre may be T13 with the same halves and row stride.  half <= N rounded up to 64, whole 16-byte chunks everywhere.
   const uint16_t* pre = nullptr;

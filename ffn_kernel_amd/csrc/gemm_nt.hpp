@@ -1393,8 +1393,8 @@ __device__ __forceinline__ void swiglu_bwd_epilogue(const GemmArgs& g, typename 
       swiglu_bwd(t1[buf][k], t3[buf][k], W::get(lds, tl.wave, tl.lane, b * BATCH + k), &o1, &o3, &oh);
       if (row >= row_end || n >= g.half) continue;
       uint16_t* dst = g.T13 + (int64_t)row * g.ld13 + n;
-      if (in) *reinterpret_cast<uint4*>(g.C + (int64_t)row * g.ldc + n) = oh;
-      else o1 = o3 = make_uint4(0, 0, 0, 0);  // (the weight rows there are others')
+      if (in && g.C != nullptr) *reinterpret_cast<uint4*>(g.C + (int64_t)row * g.ldc + n) = oh;
+      if (!in) o1 = o3 = make_uint4(0, 0, 0, 0);  // (the weight rows there are others')
       *reinterpret_cast<uint4*>(dst) = o1;
       *reinterpret_cast<uint4*>(dst + g.half) = o3;
     }

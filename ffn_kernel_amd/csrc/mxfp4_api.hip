@@ -193,7 +193,7 @@ struct FfnRoom {
 };
 FfnRoom ffn_room(int64_t M, int64_t d, int64_t h, bool tiled) {
   FfnRoom r{};
-  const bool stream = M <= kMxStreamRows && !tiled;
+  const bool stream = M <= kMxStreamFfnRows && !tiled;
   r.x = stream ? 0 : routing_bytes(M);
   r.h = r.x + tensor_bytes(M, d);
   r.p = r.h + tensor_bytes(M, h);
@@ -323,7 +323,7 @@ int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t
   if (int e = check_ws(ws, ws_bytes, room.total)) return e;
   uint8_t* wsb = static_cast<uint8_t*>(ws);
   const Room hidden = carve_tensor(wsb + room.h, M, h);
-  if (M <= kMxStreamRows && !pre) {
+  if (M <= kMxStreamFfnRows && !pre) {
     if (int e = leave_routing(routing, made, mask, M, stream)) return e;
     MxStreamArgs a{};
     if (int e = stream_rows(x, x_stride_m, xq, carve_tensor(wsb + room.x, M, d), M, d, stream, &a)) return e;

@@ -339,12 +339,14 @@ hipError_t launch_tiles(const MxStreamArgs& a, hipStream_t stream) {
 template <bool DUAL, int TILES>
 hipError_t launch(const MxStreamArgs& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  if (a.M > kMxStreamRows || a.K <= 0 || (a.x != nullptr && !mx_stream_takes(a.M, a.K, a.x, a.ldx))) return hipErrorInvalidValue;
+  if (a.M > (DUAL ? kMxStreamFfnRows : kMxStreamRows) || a.K <= 0 || (a.x != nullptr && !mx_stream_takes(a.M, a.K, a.x, a.ldx))) return hipErrorInvalidValue;
   switch (cdiv(a.M, 16)) {
     case 1: return a.x != nullptr ? launch_tiles<1, DUAL, TILES, true>(a, stream) : launch_tiles<1, DUAL, TILES, false>(a, stream);
     case 2: return launch_tiles<2, DUAL, TILES, false>(a, stream);
     case 3: return launch_tiles<3, DUAL, TILES, false>(a, stream);
-    default: return launch_tiles<4, DUAL, TILES, false>(a, stream);
+    default:
+      if constexpr (DUAL) return hipErrorInvalidValue;
+      else return launch_tiles<4, DUAL, TILES, false>(a, stream);
   }
 }
 
