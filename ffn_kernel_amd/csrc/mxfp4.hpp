@@ -142,7 +142,7 @@ struct MxGemmArgs {
   int M, N, K;
   int splits; float* P;            // single weight, splits > 1: fp32 sums of a K range at P[split][p][N]
 };
-enum MxTileId : int { MX_256x256 = 0, MX_128x256 = 1, MX_128x128 = 2, MX_64x128 = 3 };
+enum MxTileId : int { MX_256x256 = 0, MX_128x128 = 1, MX_64x128 = 2 };
 constexpr int64_t kMxMaxWorkgroups = 0xffff00;  // (2^32 threads)
 int mx_tile_rows(int tile);
 int mx_tile_columns(int tile, bool dual);  // output columns

@@ -34,12 +34,13 @@ Room carve_tensor(uint8_t* ws, int64_t rows, int64_t columns) { return {ws, ws +
 
 // Tile and K ranges of a GEMM over [M, K] x [N, K]^T: the cheapest by a model of the launch, in us.  A round of tiles (`slots` at once)
 // costs a fixed time and a time per stage of 256 columns, both at most half full and quite full, in between by its share.  The costs are
-// fits to (256x256 / 128x256 / 128x128 / 64x128, single weight, half of the rows in either modality)
-//   M 4096, N 4096, K 14336  110 / 130 / 129 / 197      M 8192, N = K = 2048  28.1 / 31.7 / 28.2 / 37.3
-//   M 1411, N 4096, K 14336  77.4 / 52.9 / 53.6 / 74.5  M 8192, N = K = 1024  18.5 / 14.3 / 12.5 / 14.7
-//   M 300, N 4096, K 14336   68.0 / 44.6 / 35.6 / 33.4  M 2048, N = K = 1024  16.2 / 10.5 / 7.6 / 6.9
-// and, with an eighth more for the smaller tiles, SwiGLU's (K = 4096, 14336 columns): M = 300 38.0 / 46.2 / 44.3 / 52.4, M = 700
-// 71.9 / 70.3 / 66.7 / 98.9, M = 1411 124.7 / 138.8 / 130.6 / 187.8.
+// fits to (256x256 / 128x128 / 64x128, single weight, half of the rows in either modality)
+//   M 4096, N 4096, K 14336  110 / 129 / 197    M 8192, N = K = 2048  28.1 / 28.2 / 37.3
+//   M 1411, N 4096, K 14336  77.4 / 53.6 / 74.5 M 8192, N = K = 1024  18.5 / 12.5 / 14.7
+//   M 300, N 4096, K 14336   68.0 / 35.6 / 33.4 M 2048, N = K = 1024  16.2 / 7.6 / 6.9
+// and, with an eighth more for the smaller tiles, SwiGLU's (K = 4096, 14336 columns): M = 300 38.0 / 44.3 / 52.4, M = 700
+// 71.9 / 66.7 / 98.9, M = 1411 124.7 / 130.6 / 187.8.  (128x256 had the least by the model in 6 of 4914
+// shapes from M 49 to 32768, and is not there.)
 // K ranges add a pass over their sums: M = 300, N 4096, K 14336 in four ranges of 128x128 26.8 and 5.0.
 struct Plan {
   int tile, splits;
@@ -48,7 +49,7 @@ struct TileCost {
   int slots;
   float fixed, stage, fixed_full, stage_full;
 };
-constexpr TileCost kTileCosts[] = {{256, 12.7f, 0.96f, 14.5f, 1.7f}, {256, 8.f, 0.63f, 11.f, 0.95f}, {512, 5.f, 0.5f, 7.5f, 1.05f}, {512, 4.5f, 0.5f, 4.f, 0.8f}};
+constexpr TileCost kTileCosts[] = {{256, 12.7f, 0.96f, 14.5f, 1.7f}, {512, 5.f, 0.5f, 7.5f, 1.05f}, {512, 4.5f, 0.5f, 4.f, 0.8f}};
 float launch_us(const TileCost& c, int64_t workgroups, float stages) {
   const float half = c.fixed + stages * c.stage, full = c.fixed_full + stages * c.stage_full;
   const float share = (float)(workgroups % c.slots) / (float)c.slots;

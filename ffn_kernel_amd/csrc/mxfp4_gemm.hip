@@ -400,18 +400,16 @@ template <bool DUAL>
 struct MxTiles {
   static constexpr int G = DUAL ? 8 : 4;
   using T0 = MxTile<256, 256, 2, 2, DUAL, G>;
-  using T1 = MxTile<128, 256, 2, 2, DUAL, G>;
-  using T2 = MxTile<128, 128, 2, 2, DUAL, G>;
-  using T3 = MxTile<64, 128, 2, 2, DUAL, G>;
+  using T1 = MxTile<128, 128, 2, 2, DUAL, G>;
+  using T2 = MxTile<64, 128, 2, 2, DUAL, G>;
 };
 
 template <bool DUAL>
 hipError_t dispatch(int tile, const MxGemmArgs& g, hipStream_t stream) {
   switch (tile) {
     case MX_256x256: return launch<typename MxTiles<DUAL>::T0>(g, stream);
-    case MX_128x256: return launch<typename MxTiles<DUAL>::T1>(g, stream);
-    case MX_128x128: return launch<typename MxTiles<DUAL>::T2>(g, stream);
-    case MX_64x128: return launch<typename MxTiles<DUAL>::T3>(g, stream);
+    case MX_128x128: return launch<typename MxTiles<DUAL>::T1>(g, stream);
+    case MX_64x128: return launch<typename MxTiles<DUAL>::T2>(g, stream);
     default: return hipErrorInvalidValue;
   }
 }
@@ -419,7 +417,7 @@ hipError_t dispatch(int tile, const MxGemmArgs& g, hipStream_t stream) {
 }  // namespace
 
 int mx_tile_rows(int tile) { return tile == MX_256x256 ? 256 : tile == MX_64x128 ? 64 : 128; }
-int mx_tile_columns(int tile, bool dual) { return (tile == MX_256x256 || tile == MX_128x256 ? 256 : 128) / (dual ? 2 : 1); }
+int mx_tile_columns(int tile, bool dual) { return (tile == MX_256x256 ? 256 : 128) / (dual ? 2 : 1); }
 
 hipError_t launch_mx_gemm(int tile, const MxGemmArgs& g, hipStream_t stream) { return dispatch<false>(tile, g, stream); }
 hipError_t launch_mx_swiglu_gemm(int tile, const MxGemmArgs& g, hipStream_t stream) { return dispatch<true>(tile, g, stream); }

@@ -122,6 +122,16 @@ def test_linear_forward_on_large_tiles(m, k, n, kind):
     within(F.masked_linear_mxfp4_forward(F.mxfp4_quantise(x), qv, qt, mask), value, bound, "rows in MXFP4")
 
 
+@pytest.mark.parametrize("m,k,n,kind", [(2048, 64, 4096, "mixed"), (2048, 100, 4098, "mixed"), (1030, 64, 2060, "text"), (65, 14336, 64, "mixed"), (49, 5120, 68, "visual"),
+                                        (66, 8190, 130, "mixed"), (66, 4100, 66, "mixed"), (150, 8200, 1284, "mixed"), (3000, 7200, 64, "mixed"), (300, 14330, 36, "text"),
+                                        (8192, 4096, 60, "mixed"), (128, 14336, 704, "mixed")])
+def test_linear_forward_on_every_tile_and_number_of_k_ranges(m, k, n, kind):
+    note(f"linear plan {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    value, bound = ref.linear(a, wv, wt, mask)
+    within(F.masked_linear_mxfp4_forward(x, qv, qt, mask), value, bound, "rows in bf16")
+
+
 @pytest.mark.parametrize("m", [5, 64, 65, 300])
 def test_linear_infinities_stay_in_their_rows(m):
     note(f"linear inf / nan {m}")
@@ -232,6 +242,14 @@ def test_ffn_infinities_stay_in_their_rows():
         within(F.masked_ffn_mxfp4_forward(x, *q, mask), value, bound, "row 2 is NaN, the others not")
 
 
+@pytest.mark.parametrize("m,d,h,kind", [(256, 64, 14336, "mixed"), (300, 72, 14340, "mixed"), (100, 64, 11008, "mixed"), (130, 136, 8200, "visual"), (65, 264, 1000, "mixed"),
+                                        (48, 1024, 1032, "mixed"), (49, 1024, 1032, "mixed"), (56, 256, 8192, "text")])
+def test_ffn_forward_on_every_tile(m, d, h, kind):
+    note(f"ffn plan {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    within(F.masked_ffn_mxfp4_forward(x, *q, mask), *ref.ffn(a, w, mask), "rows in bf16")
+
+
 # ---- gradients ----------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", ["mixed", "visual", "text"])
@@ -271,6 +289,63 @@ def test_rows_in_mxfp4_carry_no_gradient():
     x, q, mask, _, _ = ffn_case(70, 64, 64, "mixed")
     y = F.MaskedFFNMXFP4.apply(F.mxfp4_quantise(x.requires_grad_()), *q, mask)
     assert not y.requires_grad
+
+
+@pytest.mark.parametrize("m", [1, 20, 64, 65, 200, 700])
+def test_calls_from_c_and_from_python_answer_alike(m, monkeypatch):
+    note(f"call.cpp {m}")
+    from ffn_kernel_amd import mxfp4
+
+    class Nothing:
+        def __getattr__(self, name):
+            return lambda *a: NotImplemented
+
+    d, h = 264, 520
+    x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+    g = rows(m, d, 3)
+
+    def everything():
+        held = F.mxfp4_quantise(x)
+        out = [*held.parts(), F.mxfp4_dequantise(held, torch.float16)]
+        out.append(F.masked_linear_mxfp4_forward(x, q[0], q[3], mask))
+        out.append(F.masked_linear_mxfp4_forward(held, q[0], q[3], mask))
+        out.append(F.masked_linear_mxfp4_backward(out[-1], q[0], q[3], mask))
+        out += F.masked_ffn_mxfp4_forward(x, *q, mask, save_pre=True)
+        out += [F.masked_ffn_mxfp4_forward(x, *q, mask), F.masked_ffn_mxfp4_forward(held, *q, mask)]
+        out.append(F.masked_ffn_mxfp4_backward(g, *q, mask, out[7]))
+        return out
+
+    usual = everything()
+    monkeypatch.setattr(mxfp4, "_native", lambda: Nothing())
+    for i, (a, b) in enumerate(zip(usual, everything(), strict=True)):
+        assert torch.equal(a, b), i
+
+
+def test_gradients_against_differences():
+    """The layers are constant in pieces (rows are rounded to four bits), so the gradient is that of the layer without the rounding:
+    differences of the 64-bit layer over the same weights, along directions.  The rounding of the rows moves it: the rows lie on the
+    grid here, where there is none, and the intermediate's rounding does not enter."""
+    note("differences")
+    m, d, h = 40, 64, 128
+    x, q, mask, _, w = ffn_case(m, d, h, "mixed")
+    x = ref.values(x).bfloat16()
+    g = rows(m, d, 3)
+
+    def layer(t):
+        def side(w1, w2, w3):
+            a = t @ w1.T
+            return (a / (1 + torch.exp(-a)) * (t @ w3.T)) @ w2.T
+        return torch.where(mask[:, None], side(*(w[n] for n in FFN[:3])), side(*(w[n] for n in FFN[3:])))
+
+    leaf = x.clone().requires_grad_()
+    F.MaskedFFNMXFP4.apply(leaf, *q, mask).backward(g)
+    _, bound = ref.ffn_grad(g, ref.values(x), w, mask)
+    for seed in range(4):
+        v = torch.randn(m, d, generator=gen(seed), device="cuda", dtype=torch.float64)
+        e = 1e-5
+        slope = ((layer(x.double() + e * v) - layer(x.double() - e * v)) / (2 * e) * g.double()).sum(1)
+        # the central difference's own error is e^2 times a third derivative: 1e-10 of values of the slope's size, far inside 1e-6
+        assert (((leaf.grad.double() * v).sum(1) - slope).abs() <= (bound * v.abs()).sum(1) + 1e-6 * slope.abs().max()).all()
 
 
 # ---- a run of them together, as a block uses them --------------------------------------------------------------------------------
@@ -339,3 +414,59 @@ def test_graphs_and_streams(m):
         eager = block(held)
         torch.cuda.synchronize()
         assert torch.equal(replayed, eager)
+
+
+@pytest.mark.parametrize("m", [30, 150])
+def test_backward_on_another_stream_and_in_a_graph(m):
+    note(f"backward graph {m}")
+    d, h = 256, 520
+    x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+    p = F.mxfp4_quantise(weight(d, d, 2)), F.mxfp4_quantise(weight(d, d, 3))
+    g = rows(m, d, 9)
+
+    def gradient(t):
+        leaf = t.detach().requires_grad_()
+        return torch.autograd.grad(F.MaskedFFNMXFP4.apply(F.MaskedLinearMXFP4.apply(leaf, *p, mask), *q, mask), leaf, g)[0]
+
+    want = gradient(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert torch.equal(gradient(x), want)
+        held = x.clone()
+        gradient(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gradient(held)
+    for seed in (31, 32, 33):
+        held.copy_(rows(m, d, seed))
+        graph.replay()
+        replayed = out.clone()
+        eager = gradient(held)
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, eager)
+
+
+def test_two_graphs_and_a_mask_that_changes():
+    """Each graph has room of its own; a replay routes by what the mask holds by then."""
+    note("two graphs")
+    m, d, h = 150, 256, 544
+    x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+    other = rows(m, d, 5)
+    mask = mask.clone()
+    with torch.no_grad():
+        F.MaskedFFNMXFP4.apply(x, *q, mask)
+        torch.cuda.synchronize()
+        graphs = []
+        for t in (x, other):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = F.MaskedFFNMXFP4.apply(t, *q, mask)
+            graphs.append((graph, out, t))
+        for seed in (1, 2, 3):
+            mask.copy_(a_mask(m, "mixed", seed))
+            for graph, _, _ in graphs:
+                graph.replay()
+            for _, out, t in graphs:
+                assert torch.equal(out, F.masked_ffn_mxfp4_forward(t, *q, mask.clone()))
