@@ -451,14 +451,14 @@ PyObject* mx_ffn_fwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const size_t bytes = mx.workspace_bytes(FFNK_OP_FFN_FWD, c.M, d, h);
   if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
   at::Tensor y = mx_empty(c, c.M, d), pre;
-  if (save) pre = mx_empty(c, c.M, 2 * h);
+  if (save) pre = mx_empty(c, c.M, 2 * h, at::kFloat);
   Partition* r;
   if (!c.routing(p[9], p[7], &r)) return nullptr;
   at::Tensor ws = mx_workspace(c, bytes);
   if (!run("ffnk_mxfp4_ffn_fwd", [&] {
         return mx.ffn_fwd(a.rows(), a.stride(), a.held(), &w[0].t, &w[1].t, &w[2].t, &w[3].t, &w[4].t, &w[5].t,
-                          static_cast<const uint8_t*>(mask->const_data_ptr()), out(y), d, save ? out(pre) : nullptr, c.M, d, h, ws.mutable_data_ptr(),
-                          (size_t)ws.numel(), c.stream, routing_of(r), r ? r->made : 1);
+                          static_cast<const uint8_t*>(mask->const_data_ptr()), out(y), d, save ? static_cast<float*>(pre.mutable_data_ptr()) : nullptr, c.M, d, h,
+                          ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r), r ? r->made : 1);
       }))
     return nullptr;
   if (r) r->made = 1;
@@ -477,9 +477,8 @@ PyObject* mx_ffn_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   Mxfp4 w[6];
   if (!g || !mx_ffn_weights(&c, p + 1, w, d)) Py_RETURN_NOTIMPLEMENTED;
   const int64_t h = w[0].rows;
-  const at::Tensor *mask = c.mask(p[7]), *pre = c.rows(p[8], 2 * h);
-  if (pre && !pre->is_contiguous()) c.ok = false;
-  if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
+  const at::Tensor *mask = c.mask(p[7]), *pre = c.strided(p[8], at::kFloat, 2);
+  if (!pre || pre->size(0) != c.M || pre->size(1) != 2 * h || !pre->is_contiguous() || !Call::aligned(*pre) || !c.ready()) Py_RETURN_NOTIMPLEMENTED;
   const size_t bytes = mx.workspace_bytes(FFNK_OP_FFN_BWD, c.M, d, h);
   if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
   at::Tensor da = mx_empty(c, c.M, d);
@@ -489,7 +488,7 @@ PyObject* mx_ffn_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (!c.fill(r, *mask)) return nullptr;
   if (!run("ffnk_mxfp4_ffn_bwd", [&] {
         return mx.ffn_bwd(in(*g), Call::ld(*g), &w[0].t, &w[1].t, &w[2].t, &w[3].t, &w[4].t, &w[5].t, static_cast<const uint8_t*>(mask->const_data_ptr()),
-                          in(*pre), out(da), d, c.M, d, h, ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r));
+                          static_cast<const float*>(pre->const_data_ptr()), out(da), d, c.M, d, h, ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r));
       }))
     return nullptr;
   return THPVariable_Wrap(std::move(da));

@@ -1522,7 +1522,7 @@ bool ffn_dx_ok(int64_t M, int64_t d, int64_t h, int64_t g_stride_m) {
          direct_ok(2 * half, 0, 2 * half, 8);
 }
 size_t ffn_dx_bytes(int64_t M, int64_t d, int64_t h) { return plan_ffn_dx(M, d, h).total; }
-int ffn_dx(const uint16_t* g, int64_t g_stride_m, const uint16_t* pre, const uint16_t* const (&W1)[2], const uint16_t* const (&W3)[2],
+int ffn_dx(const uint16_t* g, int64_t g_stride_m, const float* pre, const uint16_t* const (&W1)[2], const uint16_t* const (&W3)[2],
            const uint16_t* const (&W2)[2], const int32_t* perm, const int32_t* counts, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t d, int64_t h,
            uint8_t* ws, hipStream_t stream) {
   const FfnDxPlan p = plan_ffn_dx(M, d, h);
@@ -1533,9 +1533,9 @@ int ffn_dx(const uint16_t* g, int64_t g_stride_m, const uint16_t* pre, const uin
   a.C = nullptr; a.ldc = h;  // (the intermediate: only weight gradients need it)
   a.perm = perm; a.counts = counts;
   a.M = (int)M; a.N = (int)h; a.K = (int)d; a.group_m = plan_group_m(TUNED_NONE, M, d, h);
-  a.pre = pre; a.ld_pre = 2 * h; a.half_pre = (int)h;
+  a.pre32 = pre; a.ld_pre = 2 * h; a.half_pre = (int)h;
   a.T13 = T13; a.ld13 = 2 * p.half; a.half = (int)p.half;
-  FFNK_HIP(launch_gather_gemm_kmajor(bwd_tile(M, h, d, true), a, stream), "dh GEMM");
+  FFNK_HIP(launch_gather_gemm_kmajor32(bwd_tile(M, h, d, true), a, stream), "dh GEMM");
   GemmArgs b;
   b.A = T13; b.lda = 2 * p.half;
   b.B0[0] = W1[0]; b.B0[1] = W1[1]; b.B1[0] = W3[0]; b.B1[1] = W3[1]; b.ldb = d;

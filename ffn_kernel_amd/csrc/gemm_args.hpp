@@ -30,10 +30,12 @@ struct GemmArgs {
   // Gather kernels only (GATHER_A, rows of C in routed order), SwiGLU backward instead of the plain result: always over K-major weights, by
   // choice over row-major ones.  With
   // dh = A B0^T, t1 = pre[row, n], t3 = pre[row, half_pre + n] (rows in routed order):
-  //   T13[row, n] = dh * t3 * silu'(t1),  T13[row, half + n] = dh * silu(t1),  C[row, n] = silu(t1) * t3   for n < N (C NULL: not stored)
+  //   T13[row, n] = dh * t3 * silu'(t1),  T13[row, half + n] = dh * silu(t1),  C[row, n] = silu(t1) * t3   for n < N
   //   T13[row, n] = T13[row, half + n] = 0                                                                 for N <= n < half
   // pre may be T13 with the same halves and row stride.  half <= N rounded up to 64, whole 16-byte chunks everywhere.
+  // The kernels with Cfg::PRE32 read pre32 instead of pre, and store T13 alone: it is rounded once, from fp32 values of both factors.
   const uint16_t* pre = nullptr;
+  const float* pre32 = nullptr;
   int64_t ld_pre = 0;
   int half_pre = 0;
   uint16_t* T13 = nullptr;
@@ -70,9 +72,10 @@ struct GemmArgs {
   float* P_tail = nullptr;
 };
 
-inline bool swiglu_bwd_args_ok(const GemmArgs& g) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(g.pre) | reinterpret_cast<uintptr_t>(g.T13) | reinterpret_cast<uintptr_t>(g.C);
-  return g.pre != nullptr && g.T13 != nullptr && at % 16 == 0 && (g.ld_pre | g.half_pre | g.ld13 | g.half | g.ldc | g.N) % 8 == 0 && g.half_pre >= g.N &&
+inline bool swiglu_bwd_args_ok(const GemmArgs& g, bool pre32 = false) {
+  const void* pre = pre32 ? static_cast<const void*>(g.pre32) : g.pre;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(pre) | reinterpret_cast<uintptr_t>(g.T13) | reinterpret_cast<uintptr_t>(g.C);
+  return pre != nullptr && (!pre32 || g.C == nullptr) && g.T13 != nullptr && at % 16 == 0 && (g.ld_pre | g.half_pre | g.ld13 | g.half | g.ldc | g.N) % 8 == 0 && g.half_pre >= g.N &&
          g.half >= g.N && g.half <= (g.N + 63) / 64 * 64 && g.ld_pre >= g.half_pre + g.N && g.ld13 >= 2 * (int64_t)g.half && g.splits == 1;
 }
 

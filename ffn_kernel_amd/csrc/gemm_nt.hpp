@@ -114,6 +114,7 @@ struct RoutedGemmCfg {
   // MFMA operands exchanged: a lane's runs of four consecutive results lie along the token panel's rows instead of the
   // weight panel's (acc_col).  Same products in the same order.  Weight-gradient kernels, see splitk_store.
   static constexpr bool SWAP = SWAP_;
+  static constexpr bool PRE32 = false;      // SwiGLU backward from fp32 pre-activations (GemmArgs::pre32), see Pre32
   static constexpr int NWAVES = WAVES_M * WAVES_N;
   // Has kernels that make the row partition themselves (GemmArgs::mask), SELF below.  Not the single-weight four-wave 256x256 tile, which has no registers left
   // and is for long contractions past a round of the chip.
@@ -161,6 +162,11 @@ struct RoutedGemmCfg {
   static_assert((BM / 8) % NWAVES == 0 && (BN / 8) % NWAVES == 0, "panel rows must split evenly over waves");
   static_assert(!DUAL || (BN / 2) % 16 == 0, "gate/up split must fall on a 16-row load group");
   static_assert(!B_KMAJOR || (DIRECT && !DUAL && BN >= 64 && BN <= 512), "K-major weights: direct path, one weight");
+};
+
+template <class Base>
+struct Pre32 : Base {
+  static constexpr bool PRE32 = true;
 };
 
 // Accumulator tile b of the wave reads B-panel rows starting here.
@@ -1393,8 +1399,8 @@ __device__ __forceinline__ void swiglu_bwd_epilogue(const GemmArgs& g, typename 
       swiglu_bwd(t1[buf][k], t3[buf][k], W::get(lds, tl.wave, tl.lane, b * BATCH + k), &o1, &o3, &oh);
       if (row >= row_end || n >= g.half) continue;
       uint16_t* dst = g.T13 + (int64_t)row * g.ld13 + n;
-      if (in && g.C != nullptr) *reinterpret_cast<uint4*>(g.C + (int64_t)row * g.ldc + n) = oh;
-      if (!in) o1 = o3 = make_uint4(0, 0, 0, 0);  // (the weight rows there are others')
+      if (in) *reinterpret_cast<uint4*>(g.C + (int64_t)row * g.ldc + n) = oh;
+      else o1 = o3 = make_uint4(0, 0, 0, 0);  // (the weight rows there are others')
       *reinterpret_cast<uint4*>(dst) = o1;
       *reinterpret_cast<uint4*>(dst + g.half) = o3;
     }
@@ -1413,6 +1419,51 @@ __device__ __forceinline__ void swiglu_bwd_epilogue(const GemmArgs& g, typename 
   }
 }
 
+// The same from fp32 pre-activations, dh as it was summed: T13 is rounded once.  Straight from the accumulators, whose runs of four columns
+// are 16 bytes of a pre-activation row; four runs' rows are on their way while four others are worked on.
+template <class Cfg>
+__device__ __forceinline__ void swiglu_bwd32_epilogue(const GemmArgs& g, const typename Cfg::Acc (&acc)[Cfg::TM][Cfg::TN], int row0, int row_end,
+                                                      int n0, const TileLanes<Cfg>& tl) {
+  constexpr int RUNS = Cfg::ACC_N / 4, PER_ROW = Cfg::TN * RUNS, BATCH = 4, BATCHES = Cfg::TM * PER_ROW / BATCH;
+  static_assert(PER_ROW % BATCH == 0, "a batch lies in one row");
+  const int p0 = row0 + tl.wm * Cfg::WTM + (int)tl.lr, c0 = n0 + tl.wn * Cfg::WTN_OUT;
+  auto column = [&](int run) { return c0 + run / RUNS * Cfg::MT + acc_col<Cfg>(4 * (run % RUNS), (int)tl.lh); };
+  f32x4_t t1[2][BATCH], t3[2][BATCH];
+  auto load = [&](int b) {
+    const int row = min(p0 + b * BATCH / PER_ROW * Cfg::MT, row_end - 1);  // (past the edges: a row and columns that exist, not stored)
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const float* src = g.pre32 + (int64_t)row * g.ld_pre + min(column(b * BATCH % PER_ROW + k), g.N - 4);
+      t1[b & 1][k] = *reinterpret_cast<const f32x4_t*>(src);
+      t3[b & 1][k] = *reinterpret_cast<const f32x4_t*>(src + g.half_pre);
+    }
+  };
+  load(0);
+#pragma unroll
+  for (int b = 0; b < BATCHES; ++b) {
+    if (b + 1 < BATCHES) load(b + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const int i = b * BATCH / PER_ROW, row = p0 + i * Cfg::MT;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int run = b * BATCH % PER_ROW + k, n = column(run);
+      const f32x4_t gate = t1[b & 1][k], up = t3[b & 1][k];
+      float r1[4], r3[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float d = acc[i][run / RUNS][4 * (run % RUNS) + e], s = 1.0f / (1.0f + __expf(-gate[e])), silu = gate[e] * s;
+        r1[e] = n < g.N ? d * up[e] * (s + silu * (1.0f - s)) : 0.f;  // (the weight rows past N are others')
+        r3[e] = n < g.N ? d * silu : 0.f;
+      }
+      if (row >= row_end || n >= g.half) continue;
+      uint16_t* dst = g.T13 + (int64_t)row * g.ld13 + n;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2bf(r1[0], r1[1]), pack2bf(r1[2], r1[3]));
+      *reinterpret_cast<uint2*>(dst + g.half) = make_uint2(pack2bf(r3[0], r3[1]), pack2bf(r3[2], r3[3]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Epilogue shared by the routed kernels.  Per accumulator tile a lane holds token row lr and the output
 // columns acc_col(v, lh), i.e. runs of four consecutive columns.
 template <class Cfg, bool SELF = false>
@@ -1424,7 +1475,10 @@ __device__ __forceinline__ void routed_epilogue(const GemmArgs& g, typename Cfg:
   const uint32_t lr = tl.lr, lh = tl.lh;
   const bool save = Cfg::DUAL && g.C_pre != nullptr;  // uniform over the launch, like all of these
   if constexpr (Cfg::GATHER_A && !Cfg::SCATTER_C && !Cfg::DUAL) {
-    if (Cfg::B_KMAJOR || g.T13 != nullptr) {
+    if constexpr (Cfg::PRE32) {
+      swiglu_bwd32_epilogue<Cfg>(g, acc, row0, row_end, n0, tl);
+      return;
+    } else if (Cfg::B_KMAJOR || g.T13 != nullptr) {
       swiglu_bwd_epilogue<Cfg>(g, acc, row0, row_end, n0, tl, lds);
       return;
     }
@@ -2005,7 +2059,7 @@ inline bool routed_gemm_args_ok(const GemmArgs& g) {
     return false;
   if (!Cfg::B_KMAJOR && g.k_switch != 0) return false;
   constexpr bool kGather = Cfg::GATHER_A && !Cfg::SCATTER_C && !Cfg::DUAL;
-  if ((g.T13 != nullptr || (kGather && Cfg::B_KMAJOR)) && !(kGather && swiglu_bwd_args_ok(g))) return false;
+  if ((g.T13 != nullptr || (kGather && Cfg::B_KMAJOR)) && !(kGather && swiglu_bwd_args_ok(g, Cfg::PRE32))) return false;
   return g.k_rows == 0 || (g.k_rows > 0 && g.k_switch == round_up64(g.k_rows, kBK) && g.K == 2 * g.k_switch);
 }
 

@@ -51,6 +51,7 @@ hipError_t launch_gather_gemm(int tile, bool direct, const GemmArgs& g, hipStrea
 hipError_t launch_linear_gemm_kmajor(int tile, const GemmArgs& g, hipStream_t stream);
 hipError_t launch_down_gemm_kmajor(int tile, const GemmArgs& g, hipStream_t stream);
 hipError_t launch_gather_gemm_kmajor(int tile, const GemmArgs& g, hipStream_t stream);
+hipError_t launch_gather_gemm_kmajor32(int tile, const GemmArgs& g, hipStream_t stream);
 // P[grp][split] = A[:, kslice] @ B[:, kslice]^T (fp32 partials; weight gradients)
 hipError_t launch_splitk_gemm(int tile, const SplitKArgs& g, hipStream_t stream);
 // The same with A read in place: [rows, R] in routed order instead of a padded transpose (SplitKArgs).

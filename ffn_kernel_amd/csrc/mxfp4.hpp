@@ -137,7 +137,7 @@ struct MxGemmArgs {
   MxRows B0[2], B1[2];             // per modality (0 = visual): weight rows [N, K]; B1: the up projection of the SwiGLU kernels
   uint16_t* C; int64_t ldc;        // single weight: bf16 [M, N], in token order
   uint8_t *H, *SH;                 // SwiGLU: the intermediate as MXFP4 [M, N], rows in routed order
-  uint16_t* pre; int64_t ld_pre;   // SwiGLU, optional: both projections in bf16, C_pre[p, n] and C_pre[p, N + n]
+  float* pre; int64_t ld_pre;      // SwiGLU, optional: both projections, pre[p, n] and pre[p, N + n]
   const int32_t *perm, *counts;
   int M, N, K;
   int splits; float* P;            // single weight, splits > 1: fp32 sums of a K range at P[split][p][N]

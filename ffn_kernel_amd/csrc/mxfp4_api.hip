@@ -307,7 +307,7 @@ int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp
 
 int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2,
                        const ffnk_mxfp4_t* W3, const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
-                       uint16_t* out, int64_t out_stride_m, uint16_t* pre, int64_t M, int64_t d, int64_t h, void* ws, size_t ws_bytes, void* stream_,
+                       uint16_t* out, int64_t out_stride_m, float* pre, int64_t M, int64_t d, int64_t h, void* ws, size_t ws_bytes, void* stream_,
                        const ffnk_routing_t* routing, int made) {
   hipStream_t stream = (hipStream_t)stream_;
   if (int e = check_call(M, d, h)) return e;
@@ -319,7 +319,7 @@ int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t
     if (int e = check_tensor(weights[i], names[i])) return e;
   if (!mask || !out) return api_fail(FFNK_E_NULL, "mask or out is NULL");
   if (!aligned(out, 2) || out_stride_m < d) return api_fail(FFNK_E_STRIDE, "out_stride_m=%lld < d=%lld, or out not 2-byte aligned", (long long)out_stride_m, (long long)d);
-  if (!aligned(pre, 2)) return api_fail(FFNK_E_ALIGN, "pre not 2-byte aligned");
+  if (!aligned(pre, 4)) return api_fail(FFNK_E_ALIGN, "pre not 4-byte aligned");
   const FfnRoom room = ffn_room(M, d, h, pre != nullptr);
   if (int e = check_ws(ws, ws_bytes, room.total)) return e;
   uint8_t* wsb = static_cast<uint8_t*>(ws);
@@ -377,7 +377,7 @@ int ffnk_mxfp4_linear_bwd(const uint16_t* g, int64_t g_stride_m, const ffnk_mxfp
 }
 
 int ffnk_mxfp4_ffn_bwd(const uint16_t* g, int64_t g_stride_m, const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
-                       const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask, const uint16_t* pre, uint16_t* dx,
+                       const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask, const float* pre, uint16_t* dx,
                        int64_t dx_stride_m, int64_t M, int64_t d, int64_t h, void* ws, size_t ws_bytes, void* stream_, const ffnk_routing_t* routing) {
   hipStream_t stream = (hipStream_t)stream_;
   if (int e = check_call(M, d, h)) return e;

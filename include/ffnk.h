@@ -475,12 +475,12 @@ FFNK_API int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const 
                                    void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing, int made);
 
 /* out[m] = Q(silu(Q(x[m]) W1^T) * (Q(x[m]) W3^T)) W2^T for visual rows, U1, U2, U3 for text rows; W1, W3 [h, d], W2 [d, h].
- * The intermediate goes from fp32 straight to MXFP4.  pre (optional, bf16 [M, 2h], 16-byte aligned where a backward reads it):
- * both projections in routed order, as ffnk_masked_ffn_fwd_save writes them. */
+ * The intermediate goes from fp32 straight to MXFP4.  pre (optional, fp32 [M, 2h], 16-byte aligned where a backward reads it):
+ * both projections, gate | up, rows in routed order. */
 FFNK_API int ffnk_mxfp4_ffn_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq,
                                 const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
                                 const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
-                                uint16_t* out, int64_t out_stride_m, uint16_t* pre, int64_t M, int64_t d, int64_t h,
+                                uint16_t* out, int64_t out_stride_m, float* pre, int64_t M, int64_t d, int64_t h,
                                 void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing, int made);
 
 /* Gradient of the rows over constant weights, the quantisations passed over (straight-through): dx[m] = g[m] W_grp.
@@ -494,7 +494,7 @@ FFNK_API int ffnk_mxfp4_linear_bwd(const uint16_t* g, int64_t g_stride_m, const 
 FFNK_API int ffnk_mxfp4_ffn_bwd(const uint16_t* g, int64_t g_stride_m,
                                 const ffnk_mxfp4_t* W1, const ffnk_mxfp4_t* W2, const ffnk_mxfp4_t* W3,
                                 const ffnk_mxfp4_t* U1, const ffnk_mxfp4_t* U2, const ffnk_mxfp4_t* U3, const uint8_t* mask,
-                                const uint16_t* pre, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t d, int64_t h,
+                                const float* pre, uint16_t* dx, int64_t dx_stride_m, int64_t M, int64_t d, int64_t h,
                                 void* ws, size_t ws_bytes, void* stream, const ffnk_routing_t* routing);
 
 #ifdef __cplusplus

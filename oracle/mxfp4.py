@@ -122,16 +122,17 @@ def linear_grad(g, wv, wt, mask):
 
 
 def _ffn_grad_rows(g, a, w1, w2, w3):
-    gate, up, _, _ = _swiglu(a, w1, w3)
+    (gate, bg), (up, bu) = product(a, w1), product(a, w3)
     dh, bdh = product(g.double(), w2.T)
     s = torch.sigmoid(gate)
     d1 = s + gate * s * (1 - s)
     d2 = (s * (1 - s) * (2 + gate * (1 - 2 * s))).abs()  # |silu''|
     dt1, dt3 = dh * up * d1, dh * gate * s
-    # dh, gate, up, dt1 and dt3 are kept in bf16: every one is off by half a step, to first order; a tenth more for the products of errors
-    bdh = stored(dh, bdh)
-    b1 = 1.1 * (bdh * (up * d1).abs() + BF16 * dt1.abs() + dh.abs() * up.abs() * d2 * BF16 * gate.abs() + BF16 * dt1.abs())
-    b3 = 1.1 * (bdh * (gate * s).abs() + dh.abs() * d1.abs() * BF16 * gate.abs() + BF16 * dt3.abs())
+    # dh, gate and up are fp32 sums, dt1 and dt3 are rounded to bf16; to first order, with a tenth more for the products of errors.  The
+    # sigmoid's exponential is good to a step, its exponent's rounding grows with the gate, and six operations follow.
+    steps = (gate.abs() + 8) * 2 * FP32
+    b1 = 1.1 * (bdh * (up * d1).abs() + dh.abs() * (d1.abs() * bu + up.abs() * (d2 * bg + steps * (s + (gate * s * (1 - s)).abs()))) + BF16 * dt1.abs())
+    b3 = 1.1 * (bdh * (gate * s).abs() + dh.abs() * (d1.abs() * bg + steps * (gate * s).abs()) + BF16 * dt3.abs())
     (x, bx), (y, by) = product(dt1, w1.T), product(dt3, w3.T)
     da = x + y
     return da, stored(da, bx + by + b1 @ w1.abs() + b3 @ w3.abs())

@@ -227,7 +227,8 @@ def test_ffn_keeps_its_projections_in_routed_order(m):
     y, pre = F.masked_ffn_mxfp4_forward(x, *q, mask, save_pre=True)
     order = torch.cat((mask.nonzero().view(-1), (~mask).nonzero().view(-1)))
     for half, names in ((0, ("w1", "u1")), (h, ("w3", "u3"))):
-        value, bound = ref.linear(a, w[names[0]], w[names[1]], mask)
+        (v, bv), (t, bt) = (ref.product(a, w[n]) for n in names)
+        value, bound = torch.where(mask[:, None], v, t), torch.where(mask[:, None], bv, bt)
         within(pre[:, half:half + h], value[order], bound[order], f"projection at {half}")
     within(y, *ref.ffn(a, w, mask), "result")
 
