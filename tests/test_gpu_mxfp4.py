@@ -132,6 +132,27 @@ def test_linear_forward_on_every_tile_and_number_of_k_ranges(m, k, n, kind):
     within(F.masked_linear_mxfp4_forward(x, qv, qt, mask), value, bound, "rows in bf16")
 
 
+def test_linear_rows_that_32_bits_do_not_reach():
+    """Codes of more than 4 GiB: the rows are quantised in routed order; rows in MXFP4 are refused."""
+    note("linear 17 GB of rows")
+    k, n, times = 8192, 40, 257
+    x, qv, qt, _, (a, wv, wt) = linear_case(4096, k, n, "mixed")
+    many = x.repeat(times, 1)
+    m = many.shape[0]
+    assert m * k // 2 > 1 << 32
+    mask = torch.rand(m, generator=gen(5), device="cuda") < 0.5
+    y = F.masked_linear_mxfp4_forward(many, qv, qt, mask).view(times, 4096, n)
+    visual = ref.linear(a, wv, wt, torch.ones(4096, dtype=torch.bool, device="cuda"))
+    text = ref.linear(a, wv, wt, torch.zeros(4096, dtype=torch.bool, device="cuda"))
+    for i in (*range(0, times, 32), times - 1):
+        value, bound = (torch.where(mask.view(times, 4096, 1)[i], v, t) for v, t in zip(visual, text))
+        within(y[i], value, bound, f"rows from {4096 * i}")
+    held = F.mxfp4_quantise(many)
+    assert torch.equal(held.codes[-4096:], F.mxfp4_quantise(x).codes)
+    with pytest.raises(ValueError, match="32-bit offsets"):
+        F.masked_linear_mxfp4_forward(held, qv, qt, mask)
+
+
 @pytest.mark.parametrize("m", [5, 64, 65, 300])
 def test_linear_infinities_stay_in_their_rows(m):
     note(f"linear inf / nan {m}")
