@@ -492,3 +492,32 @@ def test_two_graphs_and_a_mask_that_changes():
                 graph.replay()
             for _, out, t in graphs:
                 assert torch.equal(out, F.masked_ffn_mxfp4_forward(t, *q, mask.clone()))
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Each thread's calls, of other sizes and masks, are in flight with the other's."""
+    note("two threads")
+    import threading
+    jobs, failed = [], []
+    for m, d, h in ((150, 256, 544), (40, 520, 264)):
+        x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+        jobs.append((x, q, mask, F.masked_ffn_mxfp4_forward(x, *q, mask)))
+    torch.cuda.synchronize()
+
+    def work(job):
+        x, q, mask, want = job
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()), torch.no_grad():
+                outs = [F.MaskedFFNMXFP4.apply(x, *q, mask) for _ in range(30)]
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(out, want) for out in outs)
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 (shown by the test)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
