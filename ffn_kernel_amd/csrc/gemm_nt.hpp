@@ -1420,7 +1420,9 @@ __device__ __forceinline__ void swiglu_bwd_epilogue(const GemmArgs& g, typename 
 }
 
 // The same from fp32 pre-activations, dh as it was summed: T13 is rounded once.  Straight from the accumulators, whose runs of four columns
-// are 16 bytes of a pre-activation row; four runs' rows are on their way while four others are worked on.
+// are 16 bytes of a pre-activation row; four runs' rows are on their way while four others are worked on.  Bound by memory, [M, 2h] in
+// fp32 in and in bf16 out: the dh GEMM at M = 4096, d = 4096, h = 14336 takes 530 us with it, 480 from bf16 pre-activations through LDS
+// (swiglu_bwd_epilogue), whose gradient is off by 0.0034 of its norm instead of 0.0023.
 template <class Cfg>
 __device__ __forceinline__ void swiglu_bwd32_epilogue(const GemmArgs& g, const typename Cfg::Acc (&acc)[Cfg::TM][Cfg::TN], int row0, int row_end,
                                                       int n0, const TileLanes<Cfg>& tl) {
