@@ -81,35 +81,46 @@ struct MxLoop {
     last_back = (int)tl.c_log >= rest ? (uint32_t)((rest - 1 - (int)tl.c_log) * 16) : 0u;
   }
 
-  __device__ __forceinline__ void address(const MxGemmArgs& g, const TileCoord& tc, int first_stage, int end_stage) {
+  // Addresses, and the loads ahead of the first stage.  The token rows' places come from memory: all of them are asked for at once, and the
+  // weight rows' loads go out before they are there.
+  __device__ __forceinline__ void begin(const MxGemmArgs& g, const TileCoord& tc, int first_stage, int end_stage) {
     kt0 = first_stage;
     kt1 = end_stage;
     const int64_t lda = (int64_t)nb * 16;
-    // Gathered rows are addressed from the start of A (the host checks that 32 bits reach them).
-    const int64_t row0 = g.gather ? 0 : tc.row0;
+    auto a_place = [&](int r) { return min(tc.row0 + r, tc.row_end - 1); };  // rows past the group's end repeat its last one; their results are not stored
+    int place[NJA], scale_place[NS];
+#pragma unroll
+    for (int j = 0; j < NJA; ++j) place[j] = g.perm[a_place(tl.load_row(j))];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) scale_place[s] = g.perm[a_place(min(s * NW + tl.wave_s, NG - 1) * 64 + tl.lane)];
+    __builtin_amdgcn_sched_barrier(0);
     const int n_first = min(tc.n0, g.N - 1);
-    auto a_row = [&](int r) {  // rows past the group's end repeat its last one; their results are not stored
-      const int p = min(tc.row0 + r, tc.row_end - 1);
-      return g.gather ? g.perm[p] : p - tc.row0;
-    };
     auto b_row = [&](int r) { return min(tc.n0 + r, g.N - 1) - n_first; };
-    code_base[0] = g.A.codes + row0 * lda;
     code_base[1] = g.B0[tc.grp].codes + n_first * lda;
     if (Cfg::DUAL) code_base[2] = g.B1[tc.grp].codes + n_first * lda;
-#pragma unroll
-    for (int j = 0; j < NJA; ++j) off_a[j] = (uint32_t)a_row(tl.load_row(j)) * (uint32_t)lda + tl.c_log * 16;
 #pragma unroll
     for (int j = 0; j < NJB; ++j) {
       const int r = tl.load_row(j) - (Cfg::DUAL && j >= NJB / 2 ? BN / 2 : 0);
       off_b[j] = (uint32_t)b_row(r) * (uint32_t)lda + tl.c_log * 16;
     }
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int l = 0; l < NJB; ++l) load(l, 0, kt0);
+#endif
+    __builtin_amdgcn_sched_barrier(0);
+    // Gathered rows are addressed from the start of A (the host checks that 32 bits reach them).
+    const int64_t row0 = g.gather ? 0 : tc.row0;
+    auto a_row = [&](int r, int gathered) { return g.gather ? gathered : a_place(r) - tc.row0; };
+    code_base[0] = g.A.codes + row0 * lda;
+#pragma unroll
+    for (int j = 0; j < NJA; ++j) off_a[j] = (uint32_t)a_row(tl.load_row(j), place[j]) * (uint32_t)lda + tl.c_log * 16;
     // Scale rows: group q of 64, the token rows' first.
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int q = min(s * NW + tl.wave_s, NG - 1);  // (uniform)
       if (q < BM / 64) {
         scale_base[s] = g.A.scales + row0 * 16;
-        off_s[s] = (uint32_t)a_row(q * 64 + tl.lane) * 16u;
+        off_s[s] = (uint32_t)a_row(q * 64 + tl.lane, scale_place[s]) * 16u;
       } else {
         const int r = q * 64 - BM;
         const bool up = Cfg::DUAL && r >= BN / 2;
@@ -119,6 +130,14 @@ struct MxLoop {
       scale_base[s] = wave_uniform(scale_base[s]);
       scale_turn[s] = (int64_t)(q < BM / 64 ? g.M : g.N) * 16;
     }
+#if defined(__HIP_DEVICE_COMPILE__)
+    // (the rest of it, and of the second stage what the stage before would have issued)
+#pragma unroll
+    for (int l = NJB; l < LOADS + NS; ++l) load(l, 0, kt0);
+    if (kt0 + 1 < kt1)
+#pragma unroll
+      for (int l = 0; l < FIRST; ++l) load(l, 1, kt0 + 1);
+#endif
   }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -144,15 +163,6 @@ struct MxLoop {
                                                0, 0, 0);
     }
   }
-  // The loads ahead of the first stage: it whole, and of the second what the stage before would have issued.
-  __device__ __forceinline__ void head() const {
-#pragma unroll
-    for (int l = 0; l < LOADS + NS; ++l) load(l, 0, kt0);
-    if (kt0 + 1 < kt1)
-#pragma unroll
-      for (int l = 0; l < FIRST; ++l) load(l, 1, kt0 + 1);
-  }
-
   // The contraction over stages [kt0, kt1), kt0 even, whose head has been issued.
   __device__ __forceinline__ void run(f32x16_t (&acc)[TM][TN]) const {
     i32x4_t fa[2][TM], fb[2][TN];
@@ -231,7 +241,6 @@ struct MxLoop {
     }
   }
 #else
-  __device__ void head() const {}
   __device__ void run(f32x16_t (&acc)[TM][TN]) const {}
 #endif
 };
@@ -404,16 +413,22 @@ __global__ __launch_bounds__(Cfg::NT, 1) void mx_gemm_kernel(const MxGemmArgs g)
   const int nk = cdiv(g.K, kMxStageK), per_split = cdiv(cdiv(nk, 2), g.splits) * 2;  // (two stages share their scales' load)
   MxLoop<Cfg> loop;
   loop.init(g, lds);
-  loop.address(g, tc, split * per_split, min((split + 1) * per_split, nk));
-  loop.head();
+  // Where the results' rows go: asked for ahead of the contraction, which hides the round trip, where registers are left for it.
+  constexpr bool AHEAD = Cfg::BM < 256;
+  int out_rows[Cfg::TM];
+  auto ask = [&]() {
+#pragma unroll
+    for (int i = 0; i < Cfg::TM; ++i) {
+      const int p = tc.row0 + loop.tl.wm * Cfg::WTM + i * 32 + (int)loop.tl.lr;
+      const int place = Cfg::DUAL ? p : g.perm[min(p, tc.row_end - 1)];
+      out_rows[i] = p < tc.row_end ? place : -1;
+    }
+  };
+  if (AHEAD) ask();
+  loop.begin(g, tc, split * per_split, min((split + 1) * per_split, nk));
   f32x16_t acc[Cfg::TM][Cfg::TN];
   loop.run(acc);
-  int out_rows[Cfg::TM];
-#pragma unroll
-  for (int i = 0; i < Cfg::TM; ++i) {
-    const int p = tc.row0 + loop.tl.wm * Cfg::WTM + i * 32 + (int)loop.tl.lr;
-    out_rows[i] = p < tc.row_end ? (Cfg::DUAL ? p : g.perm[p]) : -1;
-  }
+  if (!AHEAD) ask();
   mx_epilogue<Cfg, KEEP>(g, tc, split, loop.tl, out_rows, acc, lds);
 }
 
