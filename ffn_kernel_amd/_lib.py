@@ -97,6 +97,7 @@ _SIGNATURES.update({
     "ffnk_mxfp4_quantise": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
     "ffnk_mxfp4_dequantise": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p]),
     "ffnk_mxfp4_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
+    "ffnk_mxfp4_workspace_bytes_linear_fwd": (c_size_t, [c_void_p, c_int64, c_int64, c_int64, c_int64]),
     "ffnk_mxfp4_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,  # x, xq, Wv, Wt, mask
                                       c_void_p, c_int64, c_int64, c_int64, c_int64,               # y, M, K, N
                                       c_void_p, c_size_t, c_void_p, c_void_p, c_int]),            # ... routing, made

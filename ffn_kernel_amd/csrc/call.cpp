@@ -39,6 +39,7 @@ struct MxLibrary {
   decltype(&ffnk_mxfp4_quantise) quantise;
   decltype(&ffnk_mxfp4_dequantise) dequantise;
   decltype(&ffnk_mxfp4_workspace_bytes) workspace_bytes;
+  decltype(&ffnk_mxfp4_workspace_bytes_linear_fwd) workspace_bytes_linear_fwd;
   decltype(&ffnk_mxfp4_linear_fwd) linear_fwd;
   decltype(&ffnk_mxfp4_linear_bwd) linear_bwd;
   decltype(&ffnk_mxfp4_ffn_fwd) ffn_fwd;
@@ -383,15 +384,16 @@ PyObject* mx_linear_fwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const at::Tensor* mask = c.mask(p[3]);
   if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
   const int64_t K = a.columns, N = b1.rows;
-  const size_t bytes = mx.workspace_bytes(FFNK_OP_LINEAR_FWD, c.M, K, N);
+  const size_t bytes = mx.workspace_bytes_linear_fwd(a.rows(), a.stride(), c.M, K, N);
   if (bytes == (size_t)-1) Py_RETURN_NOTIMPLEMENTED;
   at::Tensor y = mx_empty(c, c.M, N);
   Partition* r;
   if (!c.routing(p[4], p[3], &r)) return nullptr;
-  at::Tensor ws = mx_workspace(c, bytes);
+  at::Tensor ws;  // (its allocation is a fifth of a short call)
+  if (bytes > 0) ws = mx_workspace(c, bytes);
   if (!run("ffnk_mxfp4_linear_fwd", [&] {
         return mx.linear_fwd(a.rows(), a.stride(), a.held(), &b1.t, &b2.t, static_cast<const uint8_t*>(mask->const_data_ptr()), out(y), N, c.M, K, N,
-                             ws.mutable_data_ptr(), (size_t)ws.numel(), c.stream, routing_of(r), r ? r->made : 1);
+                             bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, c.stream, routing_of(r), r ? r->made : 1);
       }))
     return nullptr;
   if (r) r->made = 1;

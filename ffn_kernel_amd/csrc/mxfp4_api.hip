@@ -95,6 +95,7 @@ int check_rows(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, in
   return x_stride_m < K ? api_fail(FFNK_E_STRIDE, "x_stride_m=%lld < K=%lld", (long long)x_stride_m, (long long)K) : FFNK_OK;
 }
 int check_ws(const void* ws, size_t have, size_t need) {
+  if (need == 0) return FFNK_OK;
   if (!ws || have < need) return api_fail(FFNK_E_WORKSPACE, "workspace %zu < %zu bytes", have, need);
   return aligned(ws, 16) ? FFNK_OK : api_fail(FFNK_E_ALIGN, "workspace not 16-byte aligned");
 }
@@ -187,6 +188,10 @@ LinearRoom linear_room(int64_t M, int64_t K, int64_t N) {
   r.total = r.p + partial_bytes(r.plan, M, N);
   return r;
 }
+// ... of a call with these rows (x NULL: MXFP4 ones): none where a stream takes them as they are.
+size_t linear_need(const LinearRoom& room, int64_t M, int64_t K, const uint16_t* x, int64_t x_stride_m) {
+  return M <= kMxStreamRows && (x == nullptr || mx_stream_takes(M, K, x, x_stride_m)) ? 0 : room.total;
+}
 // `tiled`: on the tiled kernels whatever M is (a forward that keeps its pre-activations).
 struct FfnRoom {
   Plan up, down;
@@ -275,6 +280,10 @@ size_t ffnk_mxfp4_workspace_bytes(int op, int64_t M, int64_t K, int64_t N) {
   }
 }
 
+size_t ffnk_mxfp4_workspace_bytes_linear_fwd(const uint16_t* x, int64_t x_stride_m, int64_t M, int64_t K, int64_t N) {
+  return check_call(M, K, N) ? (size_t)-1 : linear_need(linear_room(M, K, N), M, K, x, x_stride_m);
+}
+
 int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp4_t* xq, const ffnk_mxfp4_t* Wv, const ffnk_mxfp4_t* Wt,
                           const uint8_t* mask, uint16_t* y, int64_t y_stride_m, int64_t M, int64_t K, int64_t N, void* ws, size_t ws_bytes,
                           void* stream_, const ffnk_routing_t* routing, int made) {
@@ -287,7 +296,7 @@ int ffnk_mxfp4_linear_fwd(const uint16_t* x, int64_t x_stride_m, const ffnk_mxfp
   if (!mask || !y) return api_fail(FFNK_E_NULL, "mask or y is NULL");
   if (!aligned(y, 2) || y_stride_m < N) return api_fail(FFNK_E_STRIDE, "y_stride_m=%lld < N=%lld, or y not 2-byte aligned", (long long)y_stride_m, (long long)N);
   const LinearRoom room = linear_room(M, K, N);
-  if (int e = check_ws(ws, ws_bytes, room.total)) return e;
+  if (int e = check_ws(ws, ws_bytes, linear_need(room, M, K, xq ? nullptr : x, x_stride_m))) return e;
   uint8_t* wsb = static_cast<uint8_t*>(ws);
   if (M <= kMxStreamRows) {
     if (int e = leave_routing(routing, made, mask, M, stream)) return e;

@@ -111,7 +111,7 @@ def _native():
     global _native_call
     if _native_call is None:
         module, lib = ops._native(), _lib.load()
-        names = ("quantise", "dequantise", "workspace_bytes", "linear_fwd", "linear_bwd", "ffn_fwd", "ffn_bwd")
+        names = ("quantise", "dequantise", "workspace_bytes", "workspace_bytes_linear_fwd", "linear_fwd", "linear_bwd", "ffn_fwd", "ffn_bwd")
         module.bind_mxfp4(tuple(ctypes.cast(getattr(lib, f"ffnk_mxfp4_{n}"), ctypes.c_void_p).value for n in names), MXFP4)
         _native_call = module
     return _native_call

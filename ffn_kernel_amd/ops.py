@@ -114,12 +114,36 @@ class Routing:
     counts int32[2], as ffnk_route writes them.  One partition serves every operation that runs with the
     same mask - the projections of a layer, a forward and its backward - where the reference re-tests the
     mask inside every tile of every launch (linear.py:120-149, ffn.py:61-105)."""
-    __slots__ = ("perm", "counts", "M", "_struct", "address")
+    __slots__ = ("_perm", "_counts", "_room", "M", "_struct", "address")
 
     def __init__(self, perm: torch.Tensor, counts: torch.Tensor, made: bool = True):
-        self.perm, self.counts, self.M = perm, counts, perm.shape[0]
+        self._perm, self._counts, self._room, self.M = perm, counts, None, perm.shape[0]
         self._struct = _lib.PartitionStruct(_lib.RoutingStruct(perm.data_ptr(), counts.data_ptr()), int(made))
         self.address = ctypes.addressof(self._struct)
+
+    @classmethod
+    def _unmade(cls, M: int, dev: torch.device) -> "Routing":
+        """Memory for a partition that is still to be made; its tensors are cut out when somebody asks for them (2 us of a call with a
+        new mask)."""
+        new = cls.__new__(cls)
+        new._perm = new._counts = None
+        new._room, new.M = torch.empty(M + 2, dtype=torch.int32, device=dev), M
+        at = new._room.data_ptr()
+        new._struct = _lib.PartitionStruct(_lib.RoutingStruct(at, at + 4 * M), 0)
+        new.address = ctypes.addressof(new._struct)
+        return new
+
+    @property
+    def perm(self) -> torch.Tensor:
+        if self._perm is None:
+            self._perm = self._room[:self.M]
+        return self._perm
+
+    @property
+    def counts(self) -> torch.Tensor:
+        if self._counts is None:
+            self._counts = self._room[self.M:]
+        return self._counts
 
     def ref(self):
         return ctypes.byref(self._struct.routing)
@@ -127,15 +151,14 @@ class Routing:
     def make(self, mask: torch.Tensor, stream: int) -> "Routing":
         """Fill it from `mask` on `stream`, unless that has been done."""
         if not self._struct.made:
-            _lib.check(_lib.load().ffnk_route(mask.data_ptr(), self.M, self.perm.data_ptr(), self.counts.data_ptr(), stream), "ffnk_route")
+            _lib.check(_lib.load().ffnk_route(mask.data_ptr(), self.M, self._struct.routing.perm, self._struct.routing.counts, stream), "ffnk_route")
             self._struct.made = 1
         return self
 
 
 def _room(M: int, dev: torch.device) -> Routing:
     """Memory for a partition that is still to be made."""
-    buf = torch.empty(M + 2, dtype=torch.int32, device=dev)
-    return Routing(buf[:M], buf[M:], made=False)
+    return Routing._unmade(M, dev)
 
 
 def _require_route_mask(mask) -> None:

@@ -464,6 +464,9 @@ FFNK_API int ffnk_mxfp4_dequantise(const ffnk_mxfp4_t* x, void* y, int dtype, in
 /* Scratch of the calls below (op: FFNK_OP_LINEAR_FWD, FFNK_OP_FFN_FWD, FFNK_OP_LINEAR_BWD, FFNK_OP_FFN_BWD; K = d, N = h for the
  * FFN).  (size_t)-1 for another op or invalid extents. */
 FFNK_API size_t ffnk_mxfp4_workspace_bytes(int op, int64_t M, int64_t K, int64_t N);
+/* What ffnk_mxfp4_linear_fwd needs with these rows (x NULL: MXFP4 ones), no more than the above for FFNK_OP_LINEAR_FWD: 0 where a
+ * call of few rows quantises them on its way, and its ws may be NULL. */
+FFNK_API size_t ffnk_mxfp4_workspace_bytes_linear_fwd(const uint16_t* x, int64_t x_stride_m, int64_t M, int64_t K, int64_t N);
 
 /* y[m] = Q(x[m]) (mask[m] ? Wv : Wt)^T with the weights [N, K], as nn.Linear holds them.  The rows are bf16 x, quantised in the
  * call, or MXFP4 xq (the other is NULL).  fp32 sums, bf16 result.

@@ -106,6 +106,18 @@ def test_from_parts_refuses():
         F.MXFP4.from_parts(codes, scales, 32)  # all there, but in host memory
 
 
+def test_short_linear_calls_need_no_workspace():
+    need = _lib.load().ffnk_mxfp4_workspace_bytes_linear_fwd
+    whole = _lib.load().ffnk_mxfp4_workspace_bytes
+    op = _lib.OP_LINEAR_FWD
+    assert need(1 << 20, 1024, 1, 1024, 64) == 0                             # quantised in the stream
+    assert need(None, 0, 64, 1024, 64) == 0                                  # rows in MXFP4
+    assert need((1 << 20) + 2, 1024, 1, 1024, 64) == whole(op, 1, 1024, 64)  # off 16 bytes
+    assert need(1 << 20, 1024, 64, 1024, 64) == whole(op, 64, 1024, 64)
+    assert need(None, 0, 65, 1024, 64) == whole(op, 65, 1024, 64)
+    assert need(None, 0, -1, 1024, 64) == ctypes.c_size_t(-1).value
+
+
 def test_workspace_and_refusals_of_the_c_abi():
     lib = _lib.load()
     bad = ctypes.c_size_t(-1).value
@@ -129,7 +141,8 @@ def test_workspace_and_refusals_of_the_c_abi():
     assert quantise(None, 0, 0, None, 0, 32, None) == 0
     assert dequantise(q, None, 0, 32, 1, 32, None) == E["NULL"] and dequantise(q, 0x100, 0, 8, 1, 32, None) == E["STRIDE"]
     ws = (0x4000, 1 << 30)
-    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, None, 0, None, None, 0) == E["WORKSPACE"]
+    assert linear(0x100, 64, None, q, q, 0x10, 0x100, 64, 65, 64, 64, None, 0, None, None, 0) == E["WORKSPACE"]
+    assert linear(0x102, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, None, 0, None, None, 0) == E["WORKSPACE"]
     assert linear(0x100, 64, q, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]      # x and xq
     assert linear(None, 64, None, q, q, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
     assert linear(0x100, 64, None, q, None, 0x10, 0x100, 64, 4, 64, 64, *ws, None, None, 0) == E["NULL"]
