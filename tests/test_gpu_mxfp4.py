@@ -521,3 +521,18 @@ def test_two_threads_on_streams_of_their_own():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_empty_batches_train():
+    note("empty training")
+    x, q, mask, _, _ = ffn_case(8, 64, 128, "mixed")
+    leaf = x[:0].clone().requires_grad_()
+    y = F.MaskedFFNMXFP4.apply(leaf, *q, mask[:0])
+    y = y + F.MaskedLinearMXFP4.apply(leaf, F.mxfp4_quantise(weight(64, 64, 1)), F.mxfp4_quantise(weight(64, 64, 2)), mask[:0])
+    y.sum().backward()
+    assert y.shape == (0, 64) and leaf.grad.shape == (0, 64)
+    proj = F.MaskedLinearMXFP4Module.from_module(F.MaskedLinearModule(64, 40, device="cuda"))
+    with pytest.raises(ValueError, match="multiple of 64"):  # 40 output features have no backward: said at the forward
+        proj(x.requires_grad_(), mask)
+    with torch.no_grad():
+        assert proj(x, mask).shape == (8, 40)
