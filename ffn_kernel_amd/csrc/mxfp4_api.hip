@@ -34,14 +34,12 @@ Room carve_tensor(uint8_t* ws, int64_t rows, int64_t columns) { return {ws, ws +
 
 // Tile and K ranges of a GEMM over [M, K] x [N, K]^T: the cheapest by a model of the launch, in us.  A round of tiles (`slots` at once)
 // costs a fixed time and a time per stage of 256 columns, both at most half full and quite full, in between by its share.  The costs are
-// fits to (256x256 / 128x128 / 64x128, single weight, half of the rows in either modality)
-//   M 4096, N 4096, K 14336  110 / 129 / 197    M 8192, N = K = 2048  28.1 / 28.2 / 37.3
-//   M 1411, N 4096, K 14336  77.4 / 53.6 / 74.5 M 8192, N = K = 1024  18.5 / 12.5 / 14.7
-//   M 300, N 4096, K 14336   68.0 / 35.6 / 33.4 M 2048, N = K = 1024  16.2 / 7.6 / 6.9
-// and, with an eighth more for the smaller tiles, SwiGLU's (K = 4096, 14336 columns): M = 300 38.0 / 44.3 / 52.4, M = 700
-// 71.9 / 66.7 / 98.9, M = 1411 124.7 / 130.6 / 187.8.  (128x256 had the least by the model in 6 of 4914
-// shapes from M 49 to 32768, and is not there.)
-// K ranges add a pass over their sums: M = 300, N 4096, K 14336 in four ranges of 128x128 26.8 and 5.0.
+// fits to launches that find their weights in memory, as a layer of a model does (256x256 / 128x128 / 64x128, half of the rows in either modality):
+//   N 4096, K 14336: M 300 81.6 / 48.7 / 46.5, M 700 83.5 / 50.0 / 51.6, M 1411 87.0 / 63.0 / 90.8, M 4096 107 / 132 / 197
+//   M 8192, N = K = 2048 28.1 / 28.2 / 37.3    M 2048, N = K = 1024 16.4 / 7.4 / 6.5    M 3001, N 1544, K 2056 23.5 / 15.3 / 18.8
+//   SwiGLU, K = 4096, 14336 columns: M 300 37.4 / 42.9 / 52.6, M 700 69.2 / 66.0 / 98.2, M 1411 107.5 / 123.2 / 181.3
+// (128x256 had the least by the model in 6 of 4914 shapes from M 49 to 32768, and is not there.)  K ranges add a pass over their sums:
+// N 4096, K 14336 on 128x128 in one / two / four ranges and that pass: M 300 48.7, 30.1 + 4.8, 26.0 + 6; M 1411 63.0, 69.5 + 8.
 struct Plan {
   int tile, splits;
 };
@@ -49,7 +47,7 @@ struct TileCost {
   int slots;
   float fixed, stage, fixed_full, stage_full;
 };
-constexpr TileCost kTileCosts[] = {{256, 12.7f, 0.96f, 14.5f, 1.7f}, {512, 5.f, 0.5f, 7.5f, 1.05f}, {512, 4.5f, 0.5f, 4.f, 0.8f}};
+constexpr TileCost kTileCosts[] = {{256, 12.7f, 1.2f, 14.5f, 1.7f}, {512, 5.f, 0.78f, 7.5f, 1.2f}, {512, 4.5f, 0.74f, 4.f, 0.85f}};
 float launch_us(const TileCost& c, int64_t workgroups, float stages) {
   const float half = c.fixed + stages * c.stage, full = c.fixed_full + stages * c.stage_full;
   const float share = (float)(workgroups % c.slots) / (float)c.slots;
@@ -72,7 +70,6 @@ Plan plan_gemm(bool dual, int64_t M, int64_t N, int64_t K) {
       if (per_range * (splits - 1) >= pairs) continue;  // an empty range
       const float stages = splits > 1 ? (float)(2 * per_range) : (float)cdiv64(K, 256);
       float us = (1.f - more) * launch_us(c, fewer * splits, stages) + more * launch_us(c, tiles * splits, stages);
-      if (dual && tile != MX_256x256) us *= 1.125f;
       if (splits > 1) us += 2.5f + (float)(splits * M * N) * 4.f / 4e6f;
       if (us < best_us) {
         best_us = us;
