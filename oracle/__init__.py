@@ -10,6 +10,8 @@ Contents
                  fp32 / fp64 forms of the same maths and the stable row partition.
   masked_ref.c   the same maths as plain C loops in double precision on raw bf16 bits —
                  independent of torch's matmul; built by oracle/build.py into oracle/_build/.
+  mxfp4.py       the layers over MXFP4 operands in fp64, with bounds on the kernels' rounding errors;
+                 pinned against the format's definition and by differences (tests/test_mxfp4_cpu.py).
 
 How each function is pinned (tests/test_oracle*.py):
   routing            brute force over all 2^M masks for M <= 10 against a sort-based definition
