@@ -16,11 +16,11 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from .ops import (Routing, _on_device, _require_cuda_bf16, _require_mask, _route_cache, _routing_arg, _same_device,
+from .ops import (Routing, _grad_mode, _on_device, _require_cuda_bf16, _require_mask, _route_cache, _routing_arg, _same_device,
                   _stream_ptr, _workspace)
 
 _BLOCK = 32
@@ -331,8 +331,20 @@ def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP
     return da
 
 
-def _gradient_wanted(a) -> bool:
-    return torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad
+_tracing_state, _transforms_active = torch._C._get_tracing_state, torch._C._are_functorch_transforms_active
+
+
+def _nothing_to_record(a) -> bool:
+    """Whether a forward can do without Function.apply, a third of a short call's host time.  Not where a gradient is wanted, nor where a
+    forward-mode derivative may be on its way (which Function.apply refuses), a tracer takes the call down (it would keep the
+    result's allocation alone) or a function transform is active."""
+    gradient = torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad
+    return not gradient and forward_ad._current_level < 0 and _tracing_state() is None and not _transforms_active()
+
+
+def _gradient_of_rows(ctx) -> bool:
+    """Of a forward under Function.apply, which runs with gradients switched off (ops._grad_mode)."""
+    return _grad_mode.enabled and ctx.needs_input_grad[0]
 
 
 class MaskedLinearMXFP4(Function):
@@ -340,11 +352,15 @@ class MaskedLinearMXFP4(Function):
 
     @classmethod
     def apply(cls, a, b1, b2, mask):
-        # nothing to record: a third of a short call's host time is Function.apply's
-        return super().apply(a, b1, b2, mask) if _gradient_wanted(a) else masked_linear_mxfp4_forward(a, b1, b2, mask)
+        if _nothing_to_record(a):
+            return masked_linear_mxfp4_forward(a, b1, b2, mask)
+        _grad_mode.enabled = torch.is_grad_enabled()
+        return super().apply(a, b1, b2, mask)
 
     @staticmethod
     def forward(ctx, a, b1, b2, mask):
+        if not _gradient_of_rows(ctx):
+            return masked_linear_mxfp4_forward(a, b1, b2, mask)
         if isinstance(b1, MXFP4):
             _check_differentiable(*b1.shape)
         _route_cache.last = None
@@ -368,13 +384,16 @@ class MaskedFFNMXFP4(Function):
 
     @classmethod
     def apply(cls, a, w1, w2, w3, u1, u2, u3, mask):
-        if _gradient_wanted(a):
-            return super().apply(a, w1, w2, w3, u1, u2, u3, mask)
-        return masked_ffn_mxfp4_forward(a, w1, w2, w3, u1, u2, u3, mask)
+        if _nothing_to_record(a):
+            return masked_ffn_mxfp4_forward(a, w1, w2, w3, u1, u2, u3, mask)
+        _grad_mode.enabled = torch.is_grad_enabled()
+        return super().apply(a, w1, w2, w3, u1, u2, u3, mask)
 
     @staticmethod
     def forward(ctx, a, w1, w2, w3, u1, u2, u3, mask):
         weights = (w1, w2, w3, u1, u2, u3)
+        if not _gradient_of_rows(ctx):
+            return masked_ffn_mxfp4_forward(a, *weights, mask)
         if isinstance(w2, MXFP4):
             _check_differentiable(*w2.shape)
         _route_cache.last = None

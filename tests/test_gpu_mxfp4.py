@@ -536,3 +536,31 @@ def test_empty_batches_train():
         proj(x.requires_grad_(), mask)
     with torch.no_grad():
         assert proj(x, mask).shape == (8, 40)
+
+
+# ---- what a short call skips when there is nothing to record ------------------------------------------------------------------------
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traces_replay_the_layers():
+    note("traces")
+    x, q, mask, _, _ = ffn_case(100, 64, 128, "mixed")
+    p = F.mxfp4_quantise(weight(64, 64, 2)), F.mxfp4_quantise(weight(64, 64, 3))
+
+    def block(t, m):
+        return F.MaskedFFNMXFP4.apply(F.MaskedLinearMXFP4.apply(t, *p, m), *q, m)
+
+    traced = torch.jit.trace(block, (x, mask), check_trace=False)
+    for seed in (4, 5):
+        other = rows(100, 64, seed)
+        assert torch.equal(traced(other, ~mask), block(other, ~mask))
+
+
+def test_forward_mode_is_refused():
+    note("forward mode")
+    x, q, mask, _, _ = ffn_case(100, 64, 128, "mixed")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda t: F.MaskedFFNMXFP4.apply(t, *q, mask), lambda t: F.MaskedLinearMXFP4.apply(t, q[0], q[3], mask)):
+            with pytest.raises(NotImplementedError):
+                call(dual)
+            call(x)

@@ -160,3 +160,49 @@ def test_workspace_and_refusals_of_the_c_abi():
     assert fb(0x100, 64, q, q, q, q, q, q, 0x10, None, 0x100, 64, 4, 64, 64, *ws, None, None) == E["NULL"]
     assert fb(0x100, 64, q, q, q, q, q, q, 0x10, 0x108, 0x100, 64, 4, 64, 64, *ws, None, None) == E["STRIDE"]
     assert linear(None, 0, None, None, None, None, None, 64, 0, 64, 64, None, 0, None, None, 0) == 0  # no rows
+
+
+# ---- the layers under a tracer and in forward mode: a stand-in for the foreign call, which torch cannot see into either -----------
+
+@pytest.fixture
+def unseen_layers(monkeypatch):
+    """Both forwards as functions of host memory alone: 2 a, whatever the weights."""
+    from ffn_kernel_amd import mxfp4
+
+    def twice(a, *rest, save_pre=False, **_):
+        y, held = torch.empty_like(a), 2 * a.detach()
+        ctypes.memmove(y.data_ptr(), held.data_ptr(), 4 * a.numel())
+        return (y, torch.zeros(a.shape[0], 2)) if save_pre else y
+
+    monkeypatch.setattr(mxfp4, "masked_linear_mxfp4_forward", twice)
+    monkeypatch.setattr(mxfp4, "masked_ffn_mxfp4_forward", twice)
+    return [lambda a, mask, n=n, f=f: f.apply(a, *[object()] * n, mask) for n, f in ((2, F.MaskedLinearMXFP4), (6, F.MaskedFFNMXFP4))]
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("layer", [0, 1])
+def test_a_trace_holds_the_call(unseen_layers, layer, requires_grad):
+    call, mask = unseen_layers[layer], torch.ones(3, dtype=torch.bool)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, (torch.randn(3, 4).requires_grad_(requires_grad), mask), check_trace=False)
+        for seed in (1, 2):
+            a = torch.randn(3, 4, generator=torch.Generator().manual_seed(seed))
+            held = [torch.full((3, 4), 7.0) for _ in range(64)]  # so that memory handed out anew holds something else
+            del held
+            assert torch.equal(traced(a, mask), 2 * a)
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+def test_forward_mode_is_refused(unseen_layers, layer):
+    call, mask = unseen_layers[layer], torch.ones(3, dtype=torch.bool)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(torch.randn(3, 4), torch.ones(3, 4))
+        with pytest.raises(NotImplementedError):
+            call(dual, mask)
+        plain = torch.randn(3, 4)
+        assert torch.equal(call(plain, mask), 2 * plain)  # no derivative on its way
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda a: call(a, mask), (torch.randn(3, 4),), (torch.ones(3, 4),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: call(a, mask))(torch.randn(2, 3, 4))
