@@ -206,3 +206,12 @@ def test_forward_mode_is_refused(unseen_layers, layer):
         torch.func.jvp(lambda a: call(a, mask), (torch.randn(3, 4),), (torch.ones(3, 4),))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda a: call(a, mask))(torch.randn(2, 3, 4))
+
+
+def test_conversions_refuse_a_tracer():
+    weight = torch.zeros(2, 32)
+    for convert in (F.mxfp4_quantise, lambda t: F.mxfp4_dequantise(t)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(lambda t: convert(t) or t, (torch.zeros(2, 32),), check_trace=False)
+    with pytest.raises(ValueError, match="GPU"):  # a constant of the trace: refused for where it lies alone
+        torch.jit.trace(lambda t: F.mxfp4_quantise(weight) and t, (torch.zeros(2, 32),), check_trace=False)
