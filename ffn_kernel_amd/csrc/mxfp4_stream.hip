@@ -55,6 +55,18 @@ constexpr int kFusedRows = 16, kFusedK = 8192;  // 67 KB of LDS at the most
 // h = 14336: M = 1 13.0 us, M = 16 (eight blocks) 22.4 against 20.3 and the launch.
 constexpr int kFusedBlocks = 512;
 
+// 0, which the compiler does not know: a read of LDS at an index with it may be of any slot, so the wavefront's writes ahead of it stay
+// ahead of it, and those behind it behind, also where no lane reads what it wrote itself.  The hardware runs a wavefront's LDS
+// operations in order, so the lanes then see one another's.  (A fence around the turn orders the weights' loads as well: two groups'
+// in flight take past 256 registers, d = 4096, h = 14336, both modalities, M = 27 44.5 us -> 50, M = 48 51 -> 59.)
+__device__ __forceinline__ int any_slot() {
+  int slot = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm("" : "+v"(slot));
+#endif
+  return slot;
+}
+
 // What a workgroup knows of its rows.
 struct StreamJob {
   int grp, rows;
@@ -128,9 +140,10 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
       // slot row * 16 + (piece ^ row): rows as loaded, and one piece of 16 rows, lie in different banks
 #pragma unroll
       for (int q = 0; q < 4; ++q) job.turn[(4 * q + lg) * 16 + (lr ^ (4 * q + lg))] = w.codes[r][q];
+      const int from = lr * 16 + any_slot();
       i32x4_t f[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = job.turn[lr * 16 + ((4 * i + lg) ^ lr)];
+      for (int i = 0; i < 4; ++i) f[i] = job.turn[from + ((4 * i + lg) ^ lr)];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int sw = (int)((uint32_t)w.scales[r][i] >> (8 * lg));

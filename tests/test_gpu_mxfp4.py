@@ -564,3 +564,31 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError):
                 call(dual)
             call(x)
+
+
+# ---- weight streams whose wavefronts take several 512-column groups, as many, or none -------------------------------------------------
+
+@pytest.mark.parametrize("m,k,n", [(16, 5120, 70), (9, 2600, 100), (1, 14336, 130), (16, 14330, 33), (2, 9000, 49), (27, 14336, 130), (32, 2600, 24), (20, 1544, 16),
+                                   (40, 14336, 72), (48, 7000, 31), (64, 8200, 40)])
+@pytest.mark.parametrize("kind", ["mixed", "text"])
+def test_linear_streams_of_long_rows(m, k, n, kind):
+    note(f"linear stream {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    value, bound = ref.linear(a, wv, wt, mask)
+    y = F.masked_linear_mxfp4_forward(x, qv, qt, mask)
+    within(y, value, bound, "rows in bf16")
+    within(F.masked_linear_mxfp4_forward(F.mxfp4_quantise(x), qv, qt, mask), value, bound, "rows in MXFP4")
+    assert torch.equal(y, F.masked_linear_mxfp4_forward(x, qv, qt, mask)), "the same call twice"
+
+
+@pytest.mark.parametrize("m,d,h", [(16, 4096, 264), (9, 2600, 520), (16, 5000, 40), (27, 4096, 264), (27, 2600, 136), (32, 5000, 31), (48, 4096, 136), (33, 2600, 72),
+                                   (16, 72, 9000), (27, 64, 14330), (40, 64, 8200)])
+@pytest.mark.parametrize("kind", ["mixed", "visual"])
+def test_ffn_streams_of_long_rows(m, d, h, kind):
+    note(f"ffn stream {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    value, bound = ref.ffn(a, w, mask)
+    y = F.masked_ffn_mxfp4_forward(x, *q, mask)
+    within(y, value, bound, "rows in bf16")
+    within(F.masked_ffn_mxfp4_forward(F.mxfp4_quantise(x), *q, mask), value, bound, "rows in MXFP4")
+    assert torch.equal(y, F.masked_ffn_mxfp4_forward(x, *q, mask)), "the same call twice"
