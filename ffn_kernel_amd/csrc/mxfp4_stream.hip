@@ -194,17 +194,24 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
     load_block((int)threadIdx.x);
     Weights w;
     Tokens x;
-    if (g0 + 1 < g1) {
+    // How many groups' weights are on their way meanwhile is the same for every wavefront of the workgroup, which meets in put_rows; a
+    // wavefront without that many of its own asks for the last group's again.
+    const int last = groups - 1;
+    if (per_wave > 1) {
       Weights w2;
-      load_weights(g0, w);
-      load_weights(g0 + 1, w2);
+      load_weights(min(g0, last), w);
+      load_weights(min(g0 + 1, last), w2);
       put_rows();
-      load_tokens(g0, x);
-      multiply(w, x);
-      load_tokens(g0 + 1, x);
-      multiply(w2, x);
+      if (g0 < g1) {
+        load_tokens(g0, x);
+        multiply(w, x);
+      }
+      if (g0 + 1 < g1) {
+        load_tokens(g0 + 1, x);
+        multiply(w2, x);
+      }
     } else {
-      if (g0 < g1) load_weights(g0, w);
+      load_weights(min(g0, last), w);
       put_rows();
       if (g0 < g1) {
         load_tokens(g0, x);

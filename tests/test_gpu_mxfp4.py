@@ -592,3 +592,27 @@ def test_ffn_streams_of_long_rows(m, d, h, kind):
     within(y, value, bound, "rows in bf16")
     within(F.masked_ffn_mxfp4_forward(F.mxfp4_quantise(x), *q, mask), value, bound, "rows in MXFP4")
     assert torch.equal(y, F.masked_ffn_mxfp4_forward(x, *q, mask)), "the same call twice"
+
+
+# The rows that a stream quantises itself: wavefronts with several groups, one, and none in one workgroup, up to the longest rows.
+@pytest.mark.parametrize("m,k,n", [(1, 8192, 130), (2, 8192, 70), (4, 4096, 40), (2, 6176, 33), (3, 2592, 31), (8, 2048, 24), (16, 1024, 72), (1, 544, 16)])
+@pytest.mark.parametrize("kind", ["mixed", "text"])
+def test_linear_streams_that_quantise_their_rows(m, k, n, kind):
+    note(f"linear fused stream {m}x{k}->{n} {kind}")
+    x, qv, qt, mask, (a, wv, wt) = linear_case(m, k, n, kind)
+    value, bound = ref.linear(a, wv, wt, mask)
+    y = F.masked_linear_mxfp4_forward(x, qv, qt, mask)
+    within(y, value, bound, "rows in bf16")
+    assert torch.equal(y, F.masked_linear_mxfp4_forward(F.mxfp4_quantise(x), qv, qt, mask)), "rows in MXFP4"
+
+
+@pytest.mark.parametrize("m,d,h", [(1, 4096, 1000), (4, 4096, 264), (1, 8192, 72), (2, 8192, 40), (2, 6176, 200), (1, 2592, 520), (3, 2560, 136), (5, 1568, 33),
+                                   (16, 1024, 264), (9, 1760, 96)])
+@pytest.mark.parametrize("kind", ["mixed", "visual"])
+def test_ffn_streams_that_quantise_their_rows(m, d, h, kind):
+    note(f"ffn fused stream {m} {d} {h} {kind}")
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    value, bound = ref.ffn(a, w, mask)
+    y = F.masked_ffn_mxfp4_forward(x, *q, mask)
+    within(y, value, bound, "rows in bf16")
+    assert torch.equal(y, F.masked_ffn_mxfp4_forward(F.mxfp4_quantise(x), *q, mask)), "rows in MXFP4"
