@@ -50,10 +50,11 @@ __device__ __forceinline__ i32x4_t quantise_block(const uint4 (&v)[4], uint32_t*
 // Rows in LDS: 16 bytes of codes per block and one block more, so that 16 rows' blocks lie in different banks; scales behind all rows.
 __host__ __device__ constexpr int fused_code_stride(int nb) { return (nb + 1) * 16; }
 __host__ __device__ constexpr int fused_scale_stride(int nb) { return (nb + 15) / 16 * 16 + 16; }
-constexpr int kFusedRows = 16, kFusedK = 8192;  // 67 KB of LDS at the most
+__host__ __device__ constexpr int fused_bytes(int rows, int nb) { return rows * (fused_code_stride(nb) + fused_scale_stride(nb)); }
+constexpr int kFusedRows = 16, kFusedK = 8192;
 // Every workgroup quantises all rows: worth a launch less (2.4 us) up to two blocks a thread.  SwiGLU projections, d = 4096,
 // h = 14336: M = 1 13.0 us, M = 16 (eight blocks) 22.4 against 20.3 and the launch.
-constexpr int kFusedBlocks = 512;
+constexpr int kFusedBlocks = 512;  // (9.4 KB of LDS at the most; with room for 16 rows whatever M is, M = 1, K = N = 8192 took 11.6 us, not 9.9)
 
 // 0, which the compiler does not know: a read of LDS at an index with it may be of any slot, so the wavefront's writes ahead of it stay
 // ahead of it, and those behind it behind, also where no lane reads what it wrote itself.  The hardware runs a wavefront's LDS
@@ -124,7 +125,7 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
       const uint8_t *codes, *scales;
       if constexpr (FUSED) {
         codes = job.fused + min(lr, rows - 1) * fused_code_stride(nb);
-        scales = job.fused + kFusedRows * fused_code_stride(nb) + min(lr, rows - 1) * fused_scale_stride(nb) + g * 16;
+        scales = job.fused + a.M * fused_code_stride(nb) + min(lr, rows - 1) * fused_scale_stride(nb) + g * 16;
       } else {
         codes = a.A.codes + token[t] * ld;
         scales = a.A.scales + ((int64_t)g * a.M + token[t]) * 16;
@@ -176,13 +177,13 @@ __device__ __forceinline__ void stream_body(const MxStreamArgs& a, const StreamJ
       uint32_t byte;
       const i32x4_t codes = quantise_block(v, &byte);
       *reinterpret_cast<i32x4_t*>(job.fused + r * fused_code_stride(nb) + (b - r * nb) * 16) = codes;
-      job.fused[kFusedRows * fused_code_stride(nb) + r * fused_scale_stride(nb) + (b - r * nb)] = (uint8_t)byte;
+      job.fused[a.M * fused_code_stride(nb) + r * fused_scale_stride(nb) + (b - r * nb)] = (uint8_t)byte;
     };
     auto put_rows = [&]() {
       // scale bytes behind the last block
       for (int z = (int)threadIdx.x; z < rows * pad; z += NTHREADS) {
         const int r = z / pad;
-        job.fused[kFusedRows * fused_code_stride(nb) + r * fused_scale_stride(nb) + nb + z - r * pad] = 0;
+        job.fused[a.M * fused_code_stride(nb) + r * fused_scale_stride(nb) + nb + z - r * pad] = 0;
       }
       put_block((int)threadIdx.x);
       for (int first = NTHREADS; first < blocks; first += NTHREADS) {
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(WAVES * kWave) void mx_stream_kernel(const MxStream
 template <int NT, bool DUAL, int TILES, int WAVES, bool FUSED>
 hipError_t launch_waves(const MxStreamArgs& a, hipStream_t stream) {
   const int nb = cdiv(a.K, kMxBlock);
-  const size_t lds = FUSED ? kFusedRows * (size_t)(fused_code_stride(nb) + fused_scale_stride(nb)) : 0;
+  const size_t lds = FUSED ? fused_bytes(a.M, nb) : 0;
   hipLaunchKernelGGL((mx_stream_kernel<NT, DUAL, TILES, WAVES, FUSED>), dim3((unsigned)cdiv(a.N, TILES * 16), 2), dim3(WAVES * kWave), lds, stream, a);
   return hipGetLastError();
 }
@@ -351,7 +352,7 @@ template <int NT, bool DUAL, int TILES, bool FUSED>
 hipError_t launch_tiles(const MxStreamArgs& a, hipStream_t stream) {
   const int groups = cdiv(a.K, kGroupK);
   if (groups <= 2) return launch_waves<NT, DUAL, TILES, 2, FUSED>(a, stream);
-  if constexpr (!DUAL && NT == 1)
+  if constexpr (!DUAL && NT == 1 && !FUSED)  // (FUSED: up to kFusedK)
     if (groups > 16) return launch_waves<NT, DUAL, TILES, 16, FUSED>(a, stream);
   if constexpr (!DUAL)
     if (groups > 4) return launch_waves<NT, DUAL, TILES, 8, FUSED>(a, stream);
