@@ -7,6 +7,7 @@
 // Function.apply), forward + backward 145 -> 83 (of which 76 are autograd's: its worker thread ran the Python of the backward
 // at a third of the speed); MaskedFFN forward 29.5 -> 16.0, forward + backward 259 -> 182.
 #include <Python.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
@@ -321,6 +322,7 @@ PyObject* mx_quantise(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (!t || !c.ready()) Py_RETURN_NOTIMPLEMENTED;
   const int64_t rows = t->size(0), columns = t->size(1), nb = (columns + 31) / 32;
   if (rows <= 0 || columns <= 1 || t->stride(1) != 1 || (rows > 1 && t->stride(0) < columns)) Py_RETURN_NOTIMPLEMENTED;
+  const c10::InferenceMode plain(false);  // (a backward can keep what was quantised ahead of it in any mode)
   const auto bytes = t->options().dtype(at::kByte);
   at::Tensor codes = at::empty({rows, nb * 16}, bytes), scales = at::empty({(nb + 15) / 16, rows, 16}, bytes);
   if (!run("ffnk_mxfp4_quantise", [&] {

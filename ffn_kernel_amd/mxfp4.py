@@ -66,13 +66,14 @@ class MXFP4:
         held, blocks = -(-columns // 2), -(-columns // _BLOCK)
         if columns < 0 or codes.shape[1] < held or scales.shape[1] < blocks:
             raise ValueError(f"{columns} columns need {held} bytes of codes and {blocks} scales a row, got {codes.shape[1]} and {scales.shape[1]}")
-        new_codes = torch.zeros((rows, _code_bytes(columns)), dtype=torch.uint8, device=codes.device)
-        new_scales = torch.zeros((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=codes.device)
-        new_codes[:, :held] = codes[:, :held]
-        if columns % 2:
-            new_codes[:, held - 1] &= 15
-        new_scales[:, :blocks] = scales[:, :blocks]
-        return cls(new_codes, new_scales.view(rows, -1, 16).transpose(0, 1).contiguous(), columns)
+        with torch.inference_mode(False):
+            new_codes = torch.zeros((rows, _code_bytes(columns)), dtype=torch.uint8, device=codes.device)
+            new_scales = torch.zeros((rows, -(-blocks // 16) * 16), dtype=torch.uint8, device=codes.device)
+            new_codes[:, :held] = codes[:, :held]
+            if columns % 2:
+                new_codes[:, held - 1] &= 15
+            new_scales[:, :blocks] = scales[:, :blocks]
+            return cls(new_codes, new_scales.view(rows, -1, 16).transpose(0, 1).contiguous(), columns)
 
     def parts(self) -> tuple:
         """(codes [rows, 16 ceil(columns / 32)], scales [rows, ceil(columns / 32)]): what from_parts takes, the scales as a copy."""
@@ -159,8 +160,9 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
     t = _dense_rows(t.detach())
     rows, columns = t.shape
     with _on_device(t.device):
-        codes = torch.empty((rows, _code_bytes(columns)), dtype=torch.uint8, device=t.device)
-        scales = torch.empty(_scale_shape(rows, columns), dtype=torch.uint8, device=t.device)
+        with torch.inference_mode(False):  # (a backward can keep what was quantised ahead of it in any mode)
+            codes = torch.empty((rows, _code_bytes(columns)), dtype=torch.uint8, device=t.device)
+            scales = torch.empty(_scale_shape(rows, columns), dtype=torch.uint8, device=t.device)
         q = MXFP4(codes, scales, columns)
         _lib.check(_lib.load().ffnk_mxfp4_quantise(t.data_ptr(), _DTYPES[t.dtype], _row_stride(t), q._address, rows, columns,
                                                    _stream_ptr(t.device)), "ffnk_mxfp4_quantise")
@@ -351,6 +353,20 @@ def _nothing_to_record(a) -> bool:
     return not gradient and forward_ad._current_level < 0 and _tracing_state() is None and not _transforms_active()
 
 
+def _save(ctx, weights, *tensors) -> None:
+    """For the backward: the weights' memory too, so that autograd refuses one over weights that were changed in place since."""
+    ctx.save_for_backward(*(t for w in weights for t in (w.codes, w.scales)), *tensors)
+    ctx.weights = weights
+
+
+def _saved(ctx) -> tuple:
+    """(weights, tensors) as _save got them; hooks on saved tensors may have put others in the weights' place."""
+    held, n = ctx.saved_tensors, 2 * len(ctx.weights)
+    weights = (w if codes is w.codes and scales is w.scales else MXFP4(codes, scales, w.columns)
+               for w, codes, scales in zip(ctx.weights, held[:n:2], held[1:n:2]))
+    return tuple(weights), held[n:]
+
+
 def _gradient_of_rows(ctx) -> bool:
     """Of a forward under Function.apply, which runs with gradients switched off (ops._grad_mode)."""
     return _grad_mode.enabled and ctx.needs_input_grad[0]
@@ -374,16 +390,15 @@ class MaskedLinearMXFP4(Function):
             _check_differentiable(*b1.shape)
         _route_cache.last = None
         out = masked_linear_mxfp4_forward(a, b1, b2, mask)
-        ctx.save_for_backward(mask)
-        ctx.weights = (b1, b2)
+        _save(ctx, (b1, b2), mask)
         ctx.routing = _route_cache.last
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        mask, = ctx.saved_tensors
-        return masked_linear_mxfp4_backward(grad, *ctx.weights, mask, routing=ctx.routing), None, None, None
+        weights, (mask,) = _saved(ctx)
+        return masked_linear_mxfp4_backward(grad, *weights, mask, routing=ctx.routing), None, None, None
 
 
 class MaskedFFNMXFP4(Function):
@@ -407,13 +422,12 @@ class MaskedFFNMXFP4(Function):
             _check_differentiable(*w2.shape)
         _route_cache.last = None
         out, pre = masked_ffn_mxfp4_forward(a, *weights, mask, save_pre=True)
-        ctx.save_for_backward(mask, pre)
-        ctx.weights = weights
+        _save(ctx, weights, mask, pre)
         ctx.routing = _route_cache.last
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        mask, pre = ctx.saved_tensors
-        return (masked_ffn_mxfp4_backward(grad, *ctx.weights, mask, pre, routing=ctx.routing), *([None] * 7))
+        weights, (mask, pre) = _saved(ctx)
+        return (masked_ffn_mxfp4_backward(grad, *weights, mask, pre, routing=ctx.routing), *([None] * 7))

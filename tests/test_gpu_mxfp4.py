@@ -616,3 +616,38 @@ def test_ffn_streams_that_quantise_their_rows(m, d, h, kind):
     y = F.masked_ffn_mxfp4_forward(x, *q, mask)
     within(y, value, bound, "rows in bf16")
     assert torch.equal(y, F.masked_ffn_mxfp4_forward(F.mxfp4_quantise(x), *q, mask)), "rows in MXFP4"
+
+
+def test_training_keeps_the_weights_it_ran_with():
+    note("saved weights")
+    d, h, m = 64, 128, 100
+    x, q, mask, _, _ = ffn_case(m, d, h, "mixed")
+    ffn = F.MaskedFFNMXFP4Module(d, h, device="cuda")
+    for name, w in zip(FFN, q):
+        getattr(ffn, f"{name}_codes").copy_(w.codes), getattr(ffn, f"{name}_scales").copy_(w.scales)
+    g = rows(m, d, 3)
+    leaf = x.clone().requires_grad_()
+    want, = torch.autograd.grad(ffn(leaf, mask), leaf, g)
+    with torch.autograd.graph.save_on_cpu():
+        y = ffn(leaf, mask)
+    assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
+    y = torch.utils.checkpoint.checkpoint(ffn, leaf, mask, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(y, leaf, g)[0], want)
+    y = ffn(leaf, mask)
+    ffn.load_state_dict({k: torch.zeros_like(v) for k, v in ffn.state_dict().items()})
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(g)
+
+
+def test_weights_quantised_in_inference_mode_train():
+    note("inference mode")
+    x, _, _, mask, (_, wv, wt) = linear_case(70, 128, 64, "mixed")
+    with torch.inference_mode():
+        v, t = F.mxfp4_quantise(wv.bfloat16()), F.mxfp4_quantise(wt.bfloat16())
+        t = F.MXFP4.from_parts(*t.parts(), 128)
+        narrow = F.mxfp4_quantise(torch.zeros(64, 1, device="cuda", dtype=torch.bfloat16))  # (the call that Python takes)
+    assert not any(p.is_inference() for q in (v, t, narrow) for p in (q.codes, q.scales))
+    g = rows(70, 64, 3)
+    x.requires_grad_()
+    da, = torch.autograd.grad(F.MaskedLinearMXFP4.apply(x, v, t, mask), x, g)
+    within(da, *ref.linear_grad(g.double(), wv, wt, mask), "gradient")

@@ -215,3 +215,27 @@ def test_conversions_refuse_a_tracer():
             torch.jit.trace(lambda t: convert(t) or t, (torch.zeros(2, 32),), check_trace=False)
     with pytest.raises(ValueError, match="GPU"):  # a constant of the trace: refused for where it lies alone
         torch.jit.trace(lambda t: F.mxfp4_quantise(weight) and t, (torch.zeros(2, 32),), check_trace=False)
+
+
+@pytest.mark.parametrize("layer,count", [(F.MaskedLinearMXFP4, 2), (F.MaskedFFNMXFP4, 6)])
+@pytest.mark.parametrize("part", ["codes", "scales"])
+def test_a_backward_over_changed_weights_is_refused(monkeypatch, layer, count, part):
+    from ffn_kernel_amd import mxfp4
+
+    def held():  # (an MXFP4 tensor in host memory, which its constructor refuses)
+        q = F.MXFP4.__new__(F.MXFP4)
+        q._codes, q._scales, q._columns, q._struct = torch.zeros(64, 32, dtype=torch.uint8), torch.zeros(1, 64, 16, dtype=torch.uint8), 64, None
+        return q
+
+    seen = []
+    for name in ("masked_linear_mxfp4", "masked_ffn_mxfp4"):
+        monkeypatch.setattr(mxfp4, f"{name}_forward", lambda a, *_, save_pre=False: (2 * a, torch.zeros(3, 128)) if save_pre else 2 * a)
+        monkeypatch.setattr(mxfp4, f"{name}_backward", lambda grad, *weights, **_: seen.append(weights) or 2 * grad)
+    a, mask, weights = torch.randn(3, 64, requires_grad=True), torch.ones(3, dtype=torch.bool), [held() for _ in range(count)]
+    layer.apply(a, *weights, mask).sum().backward()
+    assert torch.equal(a.grad, torch.full((3, 64), 2.0)) and all(w is q for w, q in zip(seen[0], weights))
+    for w in weights:
+        y = layer.apply(a, *weights, mask)
+        getattr(w, part).copy_(torch.ones_like(getattr(w, part)))  # what load_state_dict does
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
