@@ -82,6 +82,18 @@ class _MXFP4Weights(nn.Module):
             setattr(self, f"{name}_codes", q.codes)
             setattr(self, f"{name}_scales", q.scales)
 
+    # The MXFP4 objects of a state live as long as it does: they hold its memory.
+    def _apply(self, fn, recurse=True):
+        self._held = {}
+        return super()._apply(fn, recurse)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._held = {}
+        super()._load_from_state_dict(*args, **kwargs)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "_held": {}}
+
     def weight(self, name: str) -> MXFP4:
         codes, scales = self._buffers[f"{name}_codes"], self._buffers[f"{name}_scales"]
         held = self._held.get(name)

@@ -651,3 +651,28 @@ def test_weights_quantised_in_inference_mode_train():
     x.requires_grad_()
     da, = torch.autograd.grad(F.MaskedLinearMXFP4.apply(x, v, t, mask), x, g)
     within(da, *ref.linear_grad(g.double(), wv, wt, mask), "gradient")
+
+
+def test_a_module_that_moves_away_frees_its_weights():
+    note("offload")
+    import io
+    import weakref
+
+    x, q, mask, _, _ = ffn_case(70, 64, 128, "mixed")
+    ffn = F.MaskedFFNMXFP4Module.from_module(F.MaskedFFNModule(64, 128, device="cuda"))
+    with torch.no_grad():
+        want = ffn(x, mask)
+        gone = [weakref.ref(b) for b in ffn.buffers()]
+        ffn.cpu()
+        assert not any(ref() is not None for ref in gone)
+        assert torch.equal(ffn.cuda()(x, mask), want)
+        gone = [weakref.ref(b) for b in ffn.buffers()]
+        ffn.load_state_dict({k: v.clone() for k, v in ffn.state_dict().items()}, assign=True)
+        assert not any(ref() is not None for ref in gone)
+        assert torch.equal(ffn(x, mask), want)
+        file = io.BytesIO()
+        torch.save(ffn, file)
+        for device in ("cpu", "cuda"):
+            file.seek(0)
+            other = torch.load(file, map_location=device, weights_only=False)  # (this test's own file)
+            assert torch.equal(other.cuda()(x, mask), want)

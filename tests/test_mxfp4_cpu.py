@@ -239,3 +239,29 @@ def test_a_backward_over_changed_weights_is_refused(monkeypatch, layer, count, p
         getattr(w, part).copy_(torch.ones_like(getattr(w, part)))  # what load_state_dict does
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+def test_a_module_keeps_no_weights_of_an_earlier_state():
+    import copy
+    import pickle
+
+    module = F.MaskedLinearMXFP4Module(64, 64)
+
+    def held():
+        module._held["linear_v"] = object()  # (what a forward leaves)
+        return module._held
+
+    for change in (lambda: module.cpu(), lambda: module.to(torch.device("cpu")), lambda: module.load_state_dict(module.state_dict()),
+                   lambda: module.load_state_dict({k: torch.ones_like(v) for k, v in module.state_dict().items()}, assign=True),
+                   lambda: torch.nn.Sequential(module).float()):
+        held()
+        change()
+        assert not module._held
+    held()
+    for other in (pickle.loads(pickle.dumps(module)), copy.deepcopy(module), copy.copy(module)):
+        assert not other._held and other.state_dict().keys() == module.state_dict().keys() and other._columns == module._columns
+        assert other._held is not module._held
+    assert module._held
+    block = torch.nn.ModuleList([module])
+    block.load_state_dict(block.state_dict())
+    assert not module._held
