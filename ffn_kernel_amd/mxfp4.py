@@ -85,9 +85,10 @@ class MXFP4:
 
     @property
     def _address(self) -> int:
-        """Of its ffnk_mxfp4_t."""
+        """Of its ffnk_mxfp4_t, with the addresses that its tensors have by now (an assignment to .data gives them others)."""
         if self._struct is None:
-            self._struct = _lib.Mxfp4Struct(self._codes.data_ptr(), self._scales.data_ptr())
+            self._struct = _lib.Mxfp4Struct()
+        self._struct.codes, self._struct.scales = self._codes.data_ptr(), self._scales.data_ptr()
         return ctypes.addressof(self._struct)
 
     codes = property(lambda self: self._codes)

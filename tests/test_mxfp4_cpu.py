@@ -265,3 +265,13 @@ def test_a_module_keeps_no_weights_of_an_earlier_state():
     block = torch.nn.ModuleList([module])
     block.load_state_dict(block.state_dict())
     assert not module._held
+
+
+def test_addresses_are_those_of_the_tensors_by_then():
+    q = F.MXFP4.__new__(F.MXFP4)
+    q._codes, q._scales, q._columns, q._struct = torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(1, 2, 16, dtype=torch.uint8), 32, None
+    for _ in range(2):
+        t = _lib.Mxfp4Struct.from_address(q._address)
+        assert (t.codes, t.scales) == (q.codes.data_ptr(), q.scales.data_ptr())
+        kept = q.codes.data  # (so that the new memory is other memory)
+        q.codes.data, q.scales.data = torch.ones(2, 16, dtype=torch.uint8), torch.ones(1, 2, 16, dtype=torch.uint8)
