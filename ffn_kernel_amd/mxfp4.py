@@ -211,11 +211,19 @@ def _check_weights(K: int, dev, shape, **weights) -> None:
     _same_device(dev, **weights)
 
 
-def _check_differentiable(contraction: int, *extents: int) -> None:
-    """What the backward GEMMs over dequantised weights take; `contraction`: the layer's output features."""
-    if any(e % 8 for e in (contraction, *extents)) or (contraction % 64 and contraction < 128):
+def _reach(rows: int, stride: int, columns: int) -> bool:
+    """Whether the 32-bit offsets of the backward GEMMs span `rows` of the upstream gradient, the last one filled up to 64 columns."""
+    return 2 * (max(rows, 256) * stride + -columns % 64) < 1 << 32
+
+
+def _check_differentiable(rows: int, contraction: int, *extents: int, doubled: int = 0) -> None:
+    """What the backward GEMMs over dequantised weights take; `contraction`: the layer's output features; doubled: the intermediate's."""
+    if any(e % 8 for e in (contraction, *extents, doubled)) or (contraction % 64 and contraction < 128):
         raise ValueError(f"the MXFP4 backward needs extents that are multiples of 8 and output features that are a multiple of 64 or at "
-                         f"least 128, got {(contraction, *extents)}")
+                         f"least 128, got {(contraction, *extents, *([doubled] if doubled else []))}")
+    if not _reach(rows, contraction, contraction) or not _reach(0, 2 * (doubled + -doubled % 64), 0):
+        raise ValueError(f"the MXFP4 backward reaches 4 GiB of upstream gradient, {rows} rows of {contraction} columns pass it: split the rows"
+                         if rows > 256 else f"the MXFP4 backward has no extents as large as {max(contraction, doubled)}")
 
 
 def masked_linear_mxfp4_forward(a, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
@@ -256,7 +264,7 @@ def masked_linear_mxfp4_backward(grad: torch.Tensor, b1: MXFP4, b2: MXFP4, mask:
     if grad.shape != (M, N):
         raise ValueError(f"grad shape {tuple(grad.shape)} != {(M, N)}")
     _check_weights(K, dev, (N, K), b1=b1, b2=b2)
-    _check_differentiable(N, K)
+    _check_differentiable(M, N, K)
     mask = _require_mask(mask, M, dev)
     grad = _aligned_rows(grad)
     with _on_device(dev):
@@ -325,7 +333,7 @@ def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP
     _require_cuda_bf16("grad", grad, 2)
     M, dev = grad.shape[0], grad.device
     d, h = _check_ffn(grad.shape, dev, w1, w2, w3, u1, u2, u3)
-    _check_differentiable(d, h)
+    _check_differentiable(M, d, doubled=h)
     mask = _require_mask(mask, M, dev)
     if not isinstance(pre, torch.Tensor):
         raise TypeError(f"pre must be a torch.Tensor, got {type(pre).__name__}")
@@ -388,7 +396,7 @@ class MaskedLinearMXFP4(Function):
         if not _gradient_of_rows(ctx):
             return masked_linear_mxfp4_forward(a, b1, b2, mask)
         if isinstance(b1, MXFP4):
-            _check_differentiable(*b1.shape)
+            _check_differentiable(a.shape[:1].numel(), *b1.shape)
         _route_cache.last = None
         out = masked_linear_mxfp4_forward(a, b1, b2, mask)
         _save(ctx, (b1, b2), mask)
@@ -420,7 +428,7 @@ class MaskedFFNMXFP4(Function):
         if not _gradient_of_rows(ctx):
             return masked_ffn_mxfp4_forward(a, *weights, mask)
         if isinstance(w2, MXFP4):
-            _check_differentiable(*w2.shape)
+            _check_differentiable(a.shape[:1].numel(), w2.rows, doubled=w2.columns)
         _route_cache.last = None
         out, pre = masked_ffn_mxfp4_forward(a, *weights, mask, save_pre=True)
         _save(ctx, weights, mask, pre)

@@ -275,3 +275,35 @@ def test_addresses_are_those_of_the_tensors_by_then():
         assert (t.codes, t.scales) == (q.codes.data_ptr(), q.scales.data_ptr())
         kept = q.codes.data  # (so that the new memory is other memory)
         q.codes.data, q.scales.data = torch.ones(2, 16, dtype=torch.uint8), torch.ones(1, 2, 16, dtype=torch.uint8)
+
+
+def unheld(rows, columns):
+    """An MXFP4 tensor of these extents without memory."""
+    q = F.MXFP4.__new__(F.MXFP4)
+    q._codes, q._scales, q._columns, q._struct = torch.empty(rows, 0, dtype=torch.uint8), torch.empty(0, rows, 16, dtype=torch.uint8), columns, None
+    return q
+
+
+# A forward that keeps its rows' gradient refuses what its backward would; both go by the rule of the C ABI.
+@pytest.mark.parametrize("m,k,n", [(100, 64, 64), (524287, 512, 4096), (524288, 512, 4096), (1 << 24, 64, 64), (1 << 24, 64, 128), ((1 << 24) - 1, 64, 128),
+                                   (16777215 // 2, 8, 200), (300, 8, 1 << 23), (300, 8, (1 << 23) - 64), (256, 72, 8 * 1048575), (5, 64, 72), (5, 63, 64), (5, 72, 136)])
+def test_what_has_no_backward_is_refused_at_the_forward(m, k, n):
+    from ffn_kernel_amd import mxfp4
+
+    t = _lib.Mxfp4Struct(0x1000, 0x2000)
+    q, lib = ctypes.addressof(t), _lib.load()
+    linear = lib.ffnk_mxfp4_linear_bwd(0x100, n, q, q, 0x10, 0x100, k, m, k, n, None, 0, None, None)
+    ffn = lib.ffnk_mxfp4_ffn_bwd(0x100, n, q, q, q, q, q, q, 0x10, 0x100, 0x100, n, m, n, k, None, 0, None, None)
+    assert {linear, ffn} <= {-3, -5}  # a stride or extent that it does not take; no workspace given
+    a, mask = torch.zeros(1, requires_grad=True).bfloat16(), torch.ones(1, dtype=torch.bool)
+    up, down = unheld(k, n), unheld(n, k)
+    for code, check, call in ((linear, lambda: mxfp4._check_differentiable(m, n, k), lambda: F.MaskedLinearMXFP4.apply(a.expand(m, k), down, down, mask)),
+                              (ffn, lambda: mxfp4._check_differentiable(m, n, doubled=k),
+                               lambda: F.MaskedFFNMXFP4.apply(a.expand(m, n), up, down, up, up, down, up, mask))):
+        if code == -5:
+            check()
+            continue
+        with pytest.raises(ValueError):
+            check()
+        with pytest.raises(ValueError, match="MXFP4 backward"):
+            call()
