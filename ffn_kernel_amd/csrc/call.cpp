@@ -7,6 +7,7 @@
 // Function.apply), forward + backward 145 -> 83 (of which 76 are autograd's: its worker thread ran the Python of the backward
 // at a third of the speed); MaskedFFN forward 29.5 -> 16.0, forward + backward 259 -> 182.
 #include <Python.h>
+#include <algorithm>
 #include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -403,6 +404,11 @@ PyObject* mx_linear_fwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Rows of an upstream gradient that the backward GEMMs' 32-bit offsets span (mxfp4._reach: others are copied together, or refused).
+bool reach(const at::Tensor* g) {
+  return g && 2 * (std::max<int64_t>(g->size(0), 256) * Call::ld(*g) + (63 - (g->size(1) + 63) % 64)) < (int64_t)1 << 32;
+}
+
 // (grad, b1, b2, mask, routing) -> da
 PyObject* mx_linear_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -411,7 +417,7 @@ PyObject* mx_linear_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const int64_t N = size_of(p[0], 1);
   const at::Tensor* g = c.rows(p[0], N);
   Mxfp4 b1, b2;
-  if (!c.mxfp4(p[1], N, -1, &b1) || !c.mxfp4(p[2], N, b1.columns, &b2)) Py_RETURN_NOTIMPLEMENTED;
+  if (!reach(g) || !c.mxfp4(p[1], N, -1, &b1) || !c.mxfp4(p[2], N, b1.columns, &b2)) Py_RETURN_NOTIMPLEMENTED;
   const at::Tensor* mask = c.mask(p[3]);
   if (!c.ready()) Py_RETURN_NOTIMPLEMENTED;
   const int64_t K = b1.columns;
@@ -479,7 +485,7 @@ PyObject* mx_ffn_bwd(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const int64_t d = size_of(p[0], 1);
   const at::Tensor* g = c.rows(p[0], d);
   Mxfp4 w[6];
-  if (!g || !mx_ffn_weights(&c, p + 1, w, d)) Py_RETURN_NOTIMPLEMENTED;
+  if (!reach(g) || !mx_ffn_weights(&c, p + 1, w, d)) Py_RETURN_NOTIMPLEMENTED;
   const int64_t h = w[0].rows;
   const at::Tensor *mask = c.mask(p[7]), *pre = c.strided(p[8], at::kFloat, 2);
   if (!pre || pre->size(0) != c.M || pre->size(1) != 2 * h || !pre->is_contiguous() || !Call::aligned(*pre) || !c.ready()) Py_RETURN_NOTIMPLEMENTED;

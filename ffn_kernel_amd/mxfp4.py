@@ -281,9 +281,9 @@ def masked_linear_mxfp4_backward(grad: torch.Tensor, b1: MXFP4, b2: MXFP4, mask:
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows of a multiple of 8 columns that the direct kernels load as they are; others are copied."""
+    """Rows of a multiple of 8 columns that the direct kernels load as they are; others are copied, also those too far apart for them."""
     t = _dense_rows(t)
-    return t if _row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t if _row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0 and _reach(t.shape[0], _row_stride(t), t.shape[1]) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_ffn(a_shape, dev, w1, w2, w3, u1, u2, u3):

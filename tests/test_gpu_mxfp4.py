@@ -676,3 +676,17 @@ def test_a_module_that_moves_away_frees_its_weights():
             file.seek(0)
             other = torch.load(file, map_location=device, weights_only=False)  # (this test's own file)
             assert torch.equal(other.cuda()(x, mask), want)
+
+
+def test_upstream_gradients_whose_rows_lie_far_apart():
+    note("upstream gradient over 4.6 GB")
+    m, d, h = 1100, 64, 128
+    x, q, mask, a, w = ffn_case(m, d, h, "mixed")
+    g = rows(m, d, 3)
+    far = torch.empty(m, 1 << 21, device="cuda", dtype=torch.bfloat16)[:, 64:64 + d]
+    far.copy_(g)
+    x.requires_grad_()
+    da, = torch.autograd.grad(F.MaskedFFNMXFP4.apply(x, *q, mask), x, far)
+    within(da, *ref.ffn_grad(g, a, w, mask), "feed-forward")
+    v, t = F.mxfp4_quantise(weight(d, d, 1)), F.mxfp4_quantise(weight(d, d, 2))
+    assert torch.equal(F.masked_linear_mxfp4_backward(far, v, t, mask), F.masked_linear_mxfp4_backward(g, v, t, mask))

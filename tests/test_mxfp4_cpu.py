@@ -307,3 +307,9 @@ def test_what_has_no_backward_is_refused_at_the_forward(m, k, n):
             check()
         with pytest.raises(ValueError, match="MXFP4 backward"):
             call()
+
+
+def test_rows_far_apart_are_copied_for_the_backward():
+    from ffn_kernel_amd import mxfp4
+
+    assert mxfp4._reach(1 << 20, 2040, 128) and not mxfp4._reach(1 << 20, 2048, 128) and not mxfp4._reach(2, 1 << 23, 8)
