@@ -35,14 +35,41 @@ def _scale_shape(rows: int, columns: int) -> tuple:
     return (-(-columns // (_BLOCK * 16)), rows, 16)
 
 
+def _clear_tails(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> None:
+    """0 to what lies past the last column and the last block.  Nothing that a caller holds changes its meaning by it, so the tensors'
+    versions stay."""
+    held, blocks = -(-columns // 2), -(-columns // _BLOCK)
+    for t, any_past in ((codes, columns % _BLOCK), (scales, blocks % 16)):
+        if not any_past or t.numel() == 0:
+            continue
+        with torch.inference_mode() if t.is_inference() else torch.autograd._unsafe_preserve_version_counter(t), torch.no_grad():
+            if t is scales:
+                t[-1, :, blocks % 16:] = 0
+                continue
+            t[:, held:] = 0
+            if columns % 2:
+                t[:, held - 1] &= 15
+
+
 class MXFP4:
     """A [rows, columns] tensor in MXFP4 on a GPU: `codes` uint8 [rows, 16 ceil(columns / 32)], two elements to a byte with the even
     column in the low half, and `scales` uint8 [ceil(columns / 512), rows, 16], one exponent byte (bias 127) for 32 columns: those of
     512 columns together, and of all rows behind one another, as the products load them (parts() has them row by row).  Bytes past
-    the last column and the last block are 0: mxfp4_quantise and from_parts see to that, and the products count on it."""
+    the last column and the last block are 0, and the products count on it: the constructor sets them in the tensors that it is given."""
     __slots__ = ("_codes", "_scales", "_columns", "_struct")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
+        self._hold(codes, scales, columns)
+        _clear_tails(codes, scales, self._columns)
+
+    @classmethod
+    def _whole(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> "MXFP4":
+        """Of tensors whose last bytes are known to be 0, or still to be written."""
+        q = cls.__new__(cls)
+        q._hold(codes, scales, columns)
+        return q
+
+    def _hold(self, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> None:
         rows = codes.shape[0] if isinstance(codes, torch.Tensor) and codes.dim() == 2 else 0
         for name, t, shape in (("codes", codes, (rows, _code_bytes(columns))), ("scales", scales, _scale_shape(rows, columns))):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.shape != shape:
@@ -73,7 +100,7 @@ class MXFP4:
             if columns % 2:
                 new_codes[:, held - 1] &= 15
             new_scales[:, :blocks] = scales[:, :blocks]
-            return cls(new_codes, new_scales.view(rows, -1, 16).transpose(0, 1).contiguous(), columns)
+            return cls._whole(new_codes, new_scales.view(rows, -1, 16).transpose(0, 1).contiguous(), columns)
 
     def parts(self) -> tuple:
         """(codes [rows, 16 ceil(columns / 32)], scales [rows, ceil(columns / 32)]): what from_parts takes, the scales as a copy."""
@@ -164,7 +191,7 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
         with torch.inference_mode(False):  # (a backward can keep what was quantised ahead of it in any mode)
             codes = torch.empty((rows, _code_bytes(columns)), dtype=torch.uint8, device=t.device)
             scales = torch.empty(_scale_shape(rows, columns), dtype=torch.uint8, device=t.device)
-        q = MXFP4(codes, scales, columns)
+        q = MXFP4._whole(codes, scales, columns)
         _lib.check(_lib.load().ffnk_mxfp4_quantise(t.data_ptr(), _DTYPES[t.dtype], _row_stride(t), q._address, rows, columns,
                                                    _stream_ptr(t.device)), "ffnk_mxfp4_quantise")
     return q
@@ -371,7 +398,7 @@ def _save(ctx, weights, *tensors) -> None:
 def _saved(ctx) -> tuple:
     """(weights, tensors) as _save got them; hooks on saved tensors may have put others in the weights' place."""
     held, n = ctx.saved_tensors, 2 * len(ctx.weights)
-    weights = (w if codes is w.codes and scales is w.scales else MXFP4(codes, scales, w.columns)
+    weights = (w if codes is w.codes and scales is w.scales else MXFP4._whole(codes, scales, w.columns)
                for w, codes, scales in zip(ctx.weights, held[:n:2], held[1:n:2]))
     return tuple(weights), held[n:]
 

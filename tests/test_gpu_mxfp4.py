@@ -690,3 +690,30 @@ def test_upstream_gradients_whose_rows_lie_far_apart():
     within(da, *ref.ffn_grad(g, a, w, mask), "feed-forward")
     v, t = F.mxfp4_quantise(weight(d, d, 1)), F.mxfp4_quantise(weight(d, d, 2))
     assert torch.equal(F.masked_linear_mxfp4_backward(far, v, t, mask), F.masked_linear_mxfp4_backward(g, v, t, mask))
+
+
+@pytest.mark.parametrize("m", [5, 40, 100])
+def test_bytes_behind_the_last_block_do_not_count(m):
+    note(f"last bytes {m}")
+    d, h = 264, 1001
+    x, q, mask, a, w = ffn_case(m, d, h, "mixed")
+    value, bound = ref.ffn(a, w, mask)
+
+    def spoilt(t):
+        codes, scales = t.codes.clone(), t.scales.clone()
+        if t.columns % 32:
+            codes[:, -(-t.columns // 2):] = 0x77
+        if t.columns % 2:
+            codes[:, t.columns // 2] |= 0x70
+        blocks = -(-t.columns // 32)
+        scales[-1, :, (blocks - 1) % 16 + 1:] = 200
+        return codes, scales
+
+    bad = [F.MXFP4(*spoilt(t), t.columns) for t in q]
+    within(F.masked_ffn_mxfp4_forward(F.MXFP4(*spoilt(F.mxfp4_quantise(x)), d), *bad, mask), value, bound, "handed over")
+    ffn = F.MaskedFFNMXFP4Module(d, h, device="cuda")
+    with torch.no_grad():
+        ffn(x, mask)
+        ffn.load_state_dict({f"{n}_{part}": s for n, t in zip(FFN, q) for part, s in zip(("codes", "scales"), spoilt(t))})
+        within(ffn(x, mask), value, bound, "loaded")
+        assert torch.equal(ffn.w2_scales, q[1].scales) and torch.equal(ffn.w2_codes, q[1].codes)

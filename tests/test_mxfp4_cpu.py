@@ -313,3 +313,20 @@ def test_rows_far_apart_are_copied_for_the_backward():
     from ffn_kernel_amd import mxfp4
 
     assert mxfp4._reach(1 << 20, 2040, 128) and not mxfp4._reach(1 << 20, 2048, 128) and not mxfp4._reach(2, 1 << 23, 8)
+
+
+@pytest.mark.parametrize("columns", [0, 1, 31, 32, 33, 511, 512, 513, 1000])
+@pytest.mark.parametrize("inference", [False, True])
+def test_bytes_past_the_last_column_and_block_are_cleared(columns, inference):
+    from ffn_kernel_amd import mxfp4
+
+    with torch.inference_mode(inference):
+        codes = torch.full((3, mxfp4._code_bytes(columns)), 255, dtype=torch.uint8)
+        scales = torch.full(mxfp4._scale_shape(3, columns), 255, dtype=torch.uint8)
+    versions = None if inference else (codes._version, scales._version)
+    mxfp4._clear_tails(codes, scales, columns)
+    assert inference or (codes._version, scales._version) == versions
+    blocks = -(-columns // 32)
+    by_row, numbers = scales.transpose(0, 1).reshape(3, -1), torch.stack((codes & 15, codes >> 4), -1).view(3, -1)
+    assert (by_row[:, :blocks] == 255).all() and not by_row[:, blocks:].any()
+    assert (numbers[:, :columns] == 15).all() and not numbers[:, columns:].any()
