@@ -139,11 +139,19 @@ class Routing:
             self._perm = self._room[:self.M]
         return self._perm
 
+    @perm.setter
+    def perm(self, t: torch.Tensor) -> None:
+        self._perm, self._struct.routing.perm = t, t.data_ptr()
+
     @property
     def counts(self) -> torch.Tensor:
         if self._counts is None:
             self._counts = self._room[self.M:]
         return self._counts
+
+    @counts.setter
+    def counts(self, t: torch.Tensor) -> None:
+        self._counts, self._struct.routing.counts = t, t.data_ptr()
 
     def ref(self):
         return ctypes.byref(self._struct.routing)

@@ -330,3 +330,13 @@ def test_bytes_past_the_last_column_and_block_are_cleared(columns, inference):
     by_row, numbers = scales.transpose(0, 1).reshape(3, -1), torch.stack((codes & 15, codes >> 4), -1).view(3, -1)
     assert (by_row[:, :blocks] == 255).all() and not by_row[:, blocks:].any()
     assert (numbers[:, :columns] == 15).all() and not numbers[:, columns:].any()
+
+
+def test_tensors_of_a_partition_can_be_assigned():
+    for r in (F.Routing(torch.zeros(5, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)), F.Routing._unmade(5, torch.device("cpu"))):
+        perm, counts = torch.arange(5, dtype=torch.int32), torch.tensor([2, 3], dtype=torch.int32)
+        r.perm = perm
+        assert r.perm is perm and r.counts.shape == (2,) and r.M == 5
+        r.counts = counts
+        held = _lib.RoutingStruct.from_address(r.address)
+        assert r.counts is counts and (held.perm, held.counts) == (perm.data_ptr(), counts.data_ptr())
