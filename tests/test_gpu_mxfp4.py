@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import ffn_kernel_amd as F
+from ffn_kernel_amd import _lib
 from oracle import mxfp4 as ref
 from tests.helpers import note
 
@@ -717,3 +718,20 @@ def test_bytes_behind_the_last_block_do_not_count(m):
         ffn.load_state_dict({f"{n}_{part}": s for n, t in zip(FFN, q) for part, s in zip(("codes", "scales"), spoilt(t))})
         within(ffn(x, mask), value, bound, "loaded")
         assert torch.equal(ffn.w2_scales, q[1].scales) and torch.equal(ffn.w2_codes, q[1].codes)
+
+
+@pytest.mark.parametrize("m,d,h,kind", [(2100, 256, 6664, "mixed"), (700, 136, 264, "visual")])
+def test_gradients_on_every_tile(m, d, h, kind):
+    """The dh GEMM over fp32 projections on each tile, the big ones with a launch for what is past whole rounds, and both dx GEMMs."""
+    x, q, mask, a, w = ffn_case(m, d, h, kind)
+    g, lib = rows(m, d, 3), _lib.load()
+    _, pre = F.masked_ffn_mxfp4_forward(x, *q, mask, save_pre=True)
+    ffn, linear = ref.ffn_grad(g, a, w, mask), ref.linear_grad(g.double(), w["w2"], w["u2"], mask)
+    try:
+        for tile in (0, 1, 2, 3, 4, 6, 7):
+            note(f"gradient on tile {tile}: {m} {d} {h} {kind}")
+            lib.ffnk_debug_force_tile(tile)
+            within(F.masked_ffn_mxfp4_backward(g, *q, mask, pre), *ffn, f"feed-forward, tile {tile}")
+            within(F.masked_linear_mxfp4_backward(g, q[1], q[4], mask), *linear, f"linear, tile {tile}")
+    finally:
+        lib.ffnk_debug_force_tile(-1)
