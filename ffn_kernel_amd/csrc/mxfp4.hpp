@@ -152,8 +152,12 @@ hipError_t launch_mx_swiglu_gemm(int tile, const MxGemmArgs& g, hipStream_t stre
 // ---- mxfp4_stream.hip: up to kMxStreamRows token rows; a feed-forward layer, whose SwiGLU streams hold two weights' sums, up to
 // kMxStreamFfnRows ----
 // Streams against tiles, weights from memory, rows of one modality / of both, us: linear K = N = 4096, M = 64 10.5 / 12.6 against
-// 14.7 / 14.6; feed-forward d = 4096, h = 14336, M = 40 35.1 / 48.1 against 35.8 / 47.4, 48 37.6 / 50.0 against 36.2 / 47.7,
-// 56 45.9 / 61.0 against 36.5 / 48.5, 64 47.8 / 65.5 against 37.8 / 48.7; M = 24 32.0 / 42.0 against 35.5 / 46.9.
+// 14.7 / 14.6.  Feed-forward, 48 rows (40 rows where the tiles lead there too):
+//   d = 1024, h = 2816    13.8 / 12.4 against 18.4 / 18.5      d = 4096, h = 14336   38.9 / 51.3 against 39.0 / 48.5 (36.4 / 49.4, 38.8 / 48.0)
+//   d = 2048, h = 5632    18.7 / 18.8 against 25.6 / 26.7      d = 5120, h = 13824   54.0 / 61.3 against 44.3 / 56.3 (50.4 / 60.3, 44.1 / 56.0)
+//   d = 4096, h = 8192    26.9 / 34.4 against 33.3 / 37.0      d = 8192, h = 20480   87.1 / 119.2 against 80.4 / 138.6 (82.4 / 113.3, 79.5 / 137.4)
+// 12 % ahead at 48 rows in the geometric mean, with the tiles up to 18 % ahead; 56 rows on streams of four token tiles, which are not
+// there any more, took 45.9 / 61.0 against 36.5 / 48.5 at d = 4096, h = 14336.
 constexpr int kMxStreamRows = 64, kMxStreamFfnRows = 48;
 struct MxStreamArgs {
   MxRows A;                        // [M, K], token order

@@ -146,13 +146,13 @@ def _native():
     return _native_call
 
 
-_tracing_state, _transforms_active = torch._C._get_tracing_state, torch._C._are_functorch_transforms_active
+_tracing, _transforms_active = torch._C._is_tracing, torch._C._are_functorch_transforms_active
 
 
 def _refuse_tracer(name: str, t=None) -> None:
     """torch.jit.trace sees neither the launch nor, in an MXFP4 object, the tensors: the replays would find the traced call's codes, or
     memory that nobody wrote.  A constant of the trace (`t`) may be quantised in it."""
-    if _tracing_state() is not None and not (isinstance(t, torch.Tensor) and torch._C._get_value_trace(t).node().kind() == "prim::Constant"):
+    if not (isinstance(t, torch.Tensor) and torch._C._get_value_trace(t).node().kind() == "prim::Constant"):
         raise RuntimeError(f"{name} cannot be traced: call it ahead of torch.jit.trace (the layers' apply quantises bf16 rows and is traced whole)")
 
 
@@ -175,7 +175,8 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
     """The rows of `t` ([rows, columns], bf16, fp16 or fp32) in MXFP4, in blocks of 32 columns (ffnk_mxfp4_quantise): the scale is the
     largest power of two not above the block's largest magnitude, over 4; elements go to the nearest number, ties to the even code,
     and saturate at 6.  A block with an infinity or a NaN is NaN.  The result carries no gradient."""
-    _refuse_tracer("mxfp4_quantise", t)
+    if _tracing():
+        _refuse_tracer("mxfp4_quantise", t)
     result = _native().mx_quantise(t)
     if result is not NotImplemented:
         return result
@@ -199,7 +200,8 @@ def mxfp4_quantise(t: torch.Tensor) -> MXFP4:
 
 def mxfp4_dequantise(q: MXFP4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that `q` stands for, as a [rows, columns] tensor of bf16 (exact for normal numbers), fp16 or fp32."""
-    _refuse_tracer("mxfp4_dequantise")
+    if _tracing():
+        _refuse_tracer("mxfp4_dequantise")
     result = _native().mx_dequantise(q, dtype)
     if result is not NotImplemented:
         return result
@@ -386,7 +388,7 @@ def _nothing_to_record(a) -> bool:
     forward-mode derivative may be on its way (which Function.apply refuses), a tracer takes the call down (it would keep the
     result's allocation alone) or a function transform is active."""
     gradient = torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad
-    return not gradient and forward_ad._current_level < 0 and _tracing_state() is None and not _transforms_active()
+    return not gradient and forward_ad._current_level < 0 and not _tracing() and not _transforms_active()
 
 
 def _save(ctx, weights, *tensors) -> None:
