@@ -397,8 +397,8 @@ __device__ __forceinline__ void mx_epilogue(const MxGemmArgs& g, const TileCoord
 
 // One tile a workgroup; every XCD takes an eighth of the order.  On v_mfma_scale_f32_32x32x64_f8f6f4 (from registers alone 7.8 PFLOP/s on all
 // CUs, the 16x16x128 form 5.0).  A tile costs 11 - 14 us beyond its stages: first loads, the SwiGLU epilogue and the results.
-// M = 32768, d = 4096, h = 14336: SwiGLU 1880 - 1910 us (4.1 PFLOP/s, matrix pipes 52 % busy at a held clock of 1.84 GHz of 2.4: power),
-// down projection 800 - 870 us (4.6 PFLOP/s, 61 % at 1.73 GHz).  M = 300: 37 us for 125 MB of weights, down 26 for 62 MB and 6 for the
+// M = 32768, d = 4096, h = 14336: SwiGLU 1840 - 1910 us (4.1 PFLOP/s, matrix pipes 54 % busy at a held clock of 1.81 GHz of 2.4),
+// down projection 800 - 890 us (4.6 PFLOP/s, 61 % at 1.72 GHz).  M = 300: 38 us for 125 MB of weights, down 27 for 62 MB and 5 for the
 // sum over its K ranges: every stage waits for its weights.
 template <class Cfg, bool KEEP>
 __global__ __launch_bounds__(Cfg::NT, 1) void mx_gemm_kernel(const MxGemmArgs g) {

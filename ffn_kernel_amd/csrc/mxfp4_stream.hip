@@ -5,7 +5,7 @@
 // fetch - whole cache lines; the matrix cores' operands, 16 rows x 64 bytes, are put together in a piece of LDS of the wavefront's own
 // - and 16 scale bytes.  The token rows are the other operand: MXFP4 rows read from cache, or up to 16 bf16 rows that the workgroup
 // quantises into LDS while its weights are on their way.  The wavefronts' sums meet in LDS in a fixed order.
-// d = 4096, h = 14336: M = 1 62 MB in 13.1 us and 31 MB (down projection) in 7.5, M = 27 over both modalities 125 MB in 24.7 and 62 MB in
+// d = 4096, h = 14336: M = 1 62 MB in 13.2 us and 31 MB (down projection) in 7.7, M = 27 over both modalities 125 MB in 25 - 26 and 62 MB in
 // 15.2: 4 us to start and end, and the bytes at about 6 TB/s (6.9 from one size to the next).
 #include "mxfp4.hpp"
 

@@ -399,10 +399,11 @@ def _save(ctx, weights, *tensors) -> None:
 
 def _saved(ctx) -> tuple:
     """(weights, tensors) as _save got them; hooks on saved tensors may have put others in the weights' place."""
-    held, n = ctx.saved_tensors, 2 * len(ctx.weights)
-    weights = (w if codes is w.codes and scales is w.scales else MXFP4._whole(codes, scales, w.columns)
-               for w, codes, scales in zip(ctx.weights, held[:n:2], held[1:n:2]))
-    return tuple(weights), held[n:]
+    held, weights = ctx.saved_tensors, ctx.weights
+    pairs = [(w, held[2 * i], held[2 * i + 1]) for i, w in enumerate(weights)]
+    if any(codes is not w._codes or scales is not w._scales for w, codes, scales in pairs):
+        weights = tuple(MXFP4._whole(codes, scales, w.columns) for w, codes, scales in pairs)
+    return weights, held[2 * len(weights):]
 
 
 def _gradient_of_rows(ctx) -> bool:
