@@ -35,6 +35,16 @@ def _scale_shape(rows: int, columns: int) -> tuple:
     return (-(-columns // (_BLOCK * 16)), rows, 16)
 
 
+_tracing, _transforms_active = torch._C._is_tracing, torch._C._are_functorch_transforms_active
+
+
+def _refuse_tracer(name: str, t=None) -> None:
+    """torch.jit.trace sees neither the launch nor, in an MXFP4 object, the tensors: the replays would find the traced call's codes, or
+    memory that nobody wrote.  A constant of the trace (`t`) may be quantised in it."""
+    if not (isinstance(t, torch.Tensor) and torch._C._get_value_trace(t).node().kind() == "prim::Constant"):
+        raise RuntimeError(f"{name} cannot be traced: call it ahead of torch.jit.trace (the layers' apply quantises bf16 rows and is traced whole)")
+
+
 def _clear_tails(codes: torch.Tensor, scales: torch.Tensor, columns: int) -> None:
     """0 to what lies past the last column and the last block.  Nothing that a caller holds changes its meaning by it, so the tensors'
     versions stay."""
@@ -59,8 +69,13 @@ class MXFP4:
     __slots__ = ("_codes", "_scales", "_columns", "_struct")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int):
-        self._hold(codes, scales, columns)
-        _clear_tails(codes, scales, self._columns)
+        tracer = torch._C._get_tracing_state()
+        torch._C._set_tracing_state(None)  # (a trace keeps the object; its replays need not clear anything)
+        try:
+            self._hold(codes, scales, columns)
+            _clear_tails(codes, scales, self._columns)
+        finally:
+            torch._C._set_tracing_state(tracer)
 
     @classmethod
     def _whole(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> "MXFP4":
@@ -86,6 +101,9 @@ class MXFP4:
     def from_parts(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int | None = None) -> "MXFP4":
         """From codes [rows, at least ceil(columns / 2)] and scales [rows, at least ceil(columns / 32)] (uint8 or float8_e8m0fnu) as
         checkpoints hold them; columns: two for each byte of codes where it is not given.  Copies both."""
+        if _tracing():
+            _refuse_tracer("MXFP4.from_parts", codes)
+            _refuse_tracer("MXFP4.from_parts", scales)
         scales = scales.view(torch.uint8)
         if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[0] != scales.shape[0]:
             raise ValueError(f"codes and scales must be 8-bit [rows, ...] tensors, got {tuple(codes.shape)} and {tuple(scales.shape)}")
@@ -144,16 +162,6 @@ def _native():
         module.bind_mxfp4(tuple(ctypes.cast(getattr(lib, f"ffnk_mxfp4_{n}"), ctypes.c_void_p).value for n in names), MXFP4)
         _native_call = module
     return _native_call
-
-
-_tracing, _transforms_active = torch._C._is_tracing, torch._C._are_functorch_transforms_active
-
-
-def _refuse_tracer(name: str, t=None) -> None:
-    """torch.jit.trace sees neither the launch nor, in an MXFP4 object, the tensors: the replays would find the traced call's codes, or
-    memory that nobody wrote.  A constant of the trace (`t`) may be quantised in it."""
-    if not (isinstance(t, torch.Tensor) and torch._C._get_value_trace(t).node().kind() == "prim::Constant"):
-        raise RuntimeError(f"{name} cannot be traced: call it ahead of torch.jit.trace (the layers' apply quantises bf16 rows and is traced whole)")
 
 
 def _require_mxfp4(name: str, q) -> None:
@@ -250,9 +258,10 @@ def _check_differentiable(rows: int, contraction: int, *extents: int, doubled: i
     if any(e % 8 for e in (contraction, *extents, doubled)) or (contraction % 64 and contraction < 128):
         raise ValueError(f"the MXFP4 backward needs extents that are multiples of 8 and output features that are a multiple of 64 or at "
                          f"least 128, got {(contraction, *extents, *([doubled] if doubled else []))}")
-    if not _reach(rows, contraction, contraction) or not _reach(0, 2 * (doubled + -doubled % 64), 0):
-        raise ValueError(f"the MXFP4 backward reaches 4 GiB of upstream gradient, {rows} rows of {contraction} columns pass it: split the rows"
-                         if rows > 256 else f"the MXFP4 backward has no extents as large as {max(contraction, doubled)}")
+    if not _reach(0, contraction, contraction) or not _reach(0, 2 * (doubled + -doubled % 64), 0):
+        raise ValueError(f"the MXFP4 backward has no extents as large as {max(contraction, doubled)}")
+    if not _reach(rows, contraction, contraction):
+        raise ValueError(f"the MXFP4 backward reaches 4 GiB of upstream gradient, {rows} rows of {contraction} columns pass it: split the rows")
 
 
 def masked_linear_mxfp4_forward(a, b1: MXFP4, b2: MXFP4, mask: torch.Tensor, routing: Routing | None = None) -> torch.Tensor:
@@ -312,7 +321,9 @@ def masked_linear_mxfp4_backward(grad: torch.Tensor, b1: MXFP4, b2: MXFP4, mask:
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """Rows of a multiple of 8 columns that the direct kernels load as they are; others are copied, also those too far apart for them."""
     t = _dense_rows(t)
-    return t if _row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0 and _reach(t.shape[0], _row_stride(t), t.shape[1]) else t.clone(memory_format=torch.contiguous_format)
+    if _row_stride(t) % 8 == 0 and t.data_ptr() % 16 == 0 and _reach(t.shape[0], _row_stride(t), t.shape[1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_ffn(a_shape, dev, w1, w2, w3, u1, u2, u3):

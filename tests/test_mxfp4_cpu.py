@@ -340,3 +340,24 @@ def test_tensors_of_a_partition_can_be_assigned():
         r.counts = counts
         held = _lib.RoutingStruct.from_address(r.address)
         assert r.counts is counts and (held.perm, held.counts) == (perm.data_ptr(), counts.data_ptr())
+
+
+def test_parts_of_a_traced_value_are_refused():
+    codes, scales = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8)
+    for build in (lambda t: F.MXFP4.from_parts(t, scales, 32), lambda t: F.MXFP4.from_parts(codes, t[:, :1], 32)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(lambda t: build(t) and t, (codes,), check_trace=False)
+
+
+def test_a_trace_of_a_module_holds_no_preparation_of_its_weights(monkeypatch):
+    """Columns that end inside a group of 512: the constructor clears what lies past them, outside the trace."""
+    from ffn_kernel_amd import mxfp4
+
+    monkeypatch.setattr(F.MXFP4, "_hold", lambda self, codes, scales, columns: [setattr(self, n, v) for n, v in (
+        ("_codes", codes), ("_scales", scales), ("_columns", columns), ("_struct", None))])
+    monkeypatch.setattr(mxfp4, "masked_linear_mxfp4_forward", lambda a, *_: a.new_empty(a.shape))
+    module = F.MaskedLinearMXFP4Module(40, 40)
+    module.linear_t_scales.fill_(3)
+    traced = torch.jit.trace(module, (torch.zeros(3, 40), torch.ones(3, dtype=torch.bool)), check_trace=False)
+    assert "aten::fill_" not in str(traced.graph) and "MaskedLinearMXFP4" in str(traced.graph)
+    assert module.linear_t_scales[0, :, 2:].sum() == 0 and (module.linear_t_scales[0, :, :2] == 3).all()
