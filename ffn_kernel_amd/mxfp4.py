@@ -395,11 +395,14 @@ def masked_ffn_mxfp4_backward(grad: torch.Tensor, w1: MXFP4, w2: MXFP4, w3: MXFP
 
 
 def _nothing_to_record(a) -> bool:
-    """Whether a forward can do without Function.apply, a third of a short call's host time.  Not where a gradient is wanted, nor where a
-    forward-mode derivative may be on its way (which Function.apply refuses), a tracer takes the call down (it would keep the
-    result's allocation alone) or a function transform is active."""
-    gradient = torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad
-    return not gradient and forward_ad._current_level < 0 and not _tracing() and not _transforms_active()
+    """Whether a forward can do without Function.apply, a third of a short call's host time.  Not where a gradient of `a` is wanted, nor where
+    a tracer takes the call down (it would keep the result's allocation alone), `a` carries a forward-mode derivative or belongs to a
+    function transform (which Function.apply refuses)."""
+    if torch.is_grad_enabled() and isinstance(a, torch.Tensor) and a.requires_grad or _tracing():
+        return False
+    if forward_ad._current_level < 0 and not _transforms_active() or not isinstance(a, torch.Tensor):
+        return True
+    return not torch._C._functorch.is_functorch_wrapped_tensor(a) and (forward_ad._current_level < 0 or forward_ad.unpack_dual(a).tangent is None)
 
 
 def _save(ctx, weights, *tensors) -> None:

@@ -361,3 +361,17 @@ def test_a_trace_of_a_module_holds_no_preparation_of_its_weights(monkeypatch):
     traced = torch.jit.trace(module, (torch.zeros(3, 40), torch.ones(3, dtype=torch.bool)), check_trace=False)
     assert "aten::fill_" not in str(traced.graph) and "MaskedLinearMXFP4" in str(traced.graph)
     assert module.linear_t_scales[0, :, 2:].sum() == 0 and (module.linear_t_scales[0, :, :2] == 3).all()
+
+
+@pytest.mark.parametrize("layer", [0, 1])
+def test_transforms_of_something_else_let_the_layers_run(unseen_layers, layer):
+    call, mask, a = unseen_layers[layer], torch.ones(3, dtype=torch.bool), torch.randn(3, 4)
+    beside = lambda t: (call(a, mask) * t).sum()
+    t = torch.randn(3, 4)
+    assert torch.equal(torch.func.vmap(beside)(torch.stack((t, t)))[1], (2 * a * t).sum())
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(t, torch.ones(3, 4))
+        assert torch.equal(torch.autograd.forward_ad.unpack_dual(beside(dual)).tangent, (2 * a).sum())
+    for transform in (torch.func.grad(beside), lambda t: torch.func.jvp(beside, (t,), (torch.ones(3, 4),))):
+        with pytest.raises(RuntimeError):  # what they allocate in there has no memory
+            transform(t)
