@@ -141,6 +141,7 @@ class Routing:
 
     @perm.setter
     def perm(self, t: torch.Tensor) -> None:
+        self._check("perm", t, self.M)
         self._perm, self._struct.routing.perm = t, t.data_ptr()
 
     @property
@@ -151,7 +152,13 @@ class Routing:
 
     @counts.setter
     def counts(self, t: torch.Tensor) -> None:
+        self._check("counts", t, 2)
         self._counts, self._struct.routing.counts = t, t.data_ptr()
+
+    def _check(self, name: str, t: torch.Tensor, n: int) -> None:
+        dev = (self._room if self._room is not None else self._perm).device
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"routing: {name} must be a contiguous int32 [{n}] tensor on {dev}")
 
     def ref(self):
         return ctypes.byref(self._struct.routing)

@@ -375,3 +375,11 @@ def test_transforms_of_something_else_let_the_layers_run(unseen_layers, layer):
     for transform in (torch.func.grad(beside), lambda t: torch.func.jvp(beside, (t,), (torch.ones(3, 4),))):
         with pytest.raises(RuntimeError):  # what they allocate in there has no memory
             transform(t)
+
+
+def test_tensors_that_do_not_fit_a_partition_are_refused():
+    r = F.Routing._unmade(5, torch.device("cpu"))
+    for name, t in (("perm", torch.zeros(4, dtype=torch.int32)), ("perm", torch.zeros(5, dtype=torch.int64)), ("perm", torch.zeros(10, dtype=torch.int32)[::2]),
+                    ("counts", torch.zeros(1, dtype=torch.int32)), ("counts", [2, 3]), ("counts", torch.zeros(2, dtype=torch.int32, device="meta"))):
+        with pytest.raises(ValueError, match=name):
+            setattr(r, name, t)
